@@ -43,7 +43,7 @@ void attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, at:
   d.status = status.has_value() ? status->data_ptr<int>() : nullptr;
   d.variant = static_cast<int>(variant);
   const int rc = olb_attn_fwd(&d, cur_stream());
-  TORCH_CHECK(rc == 0, "olb_attn_fwd failed with code ", rc);
+  TORCH_CHECK(rc == 0, "olb_attn_fwd failed with code " + std::to_string(rc));
 }
 
 }  // namespace

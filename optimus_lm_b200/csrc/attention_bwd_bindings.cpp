@@ -45,7 +45,7 @@ void attn_bwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, con
   d.scale = static_cast<float>(scale);
   d.status = status.has_value() ? status->data_ptr<int>() : nullptr;
   const int rc = olb_attn_bwd(&d, at::cuda::getCurrentCUDAStream().stream());
-  TORCH_CHECK(rc == 0, "olb_attn_bwd failed with code ", rc);
+  TORCH_CHECK(rc == 0, "olb_attn_bwd failed with code " + std::to_string(rc));
 }
 
 }  // namespace

@@ -11,7 +11,7 @@ namespace {
 inline cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
 inline void check(int rc, const char* what) {
-  TORCH_CHECK(rc == 0, what, " failed with code ", rc);
+  TORCH_CHECK(rc == 0, std::string(what) + " failed with code " + std::to_string(rc));
 }
 
 #define CHECK_CUDA_BF16(t) TORCH_CHECK((t).is_cuda() && (t).scalar_type() == at::kBFloat16, #t " must be a CUDA bf16 tensor")

@@ -11,7 +11,7 @@
 namespace {
 
 inline cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
-inline void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed with code ", rc); }
+inline void check(int rc, const char* what) { TORCH_CHECK(rc == 0, std::string(what) + " failed with code " + std::to_string(rc)); }
 
 std::vector<const void*> cptrs(const std::vector<int64_t>& v) {
   std::vector<const void*> out;

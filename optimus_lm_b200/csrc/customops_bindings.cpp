@@ -14,7 +14,7 @@
 namespace {
 
 inline cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
-inline void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed with code ", rc); }
+inline void check(int rc, const char* what) { TORCH_CHECK(rc == 0, std::string(what) + " failed with code " + std::to_string(rc)); }
 
 inline bool is_f32(const at::Tensor& t) {
   TORCH_CHECK(t.is_cuda() && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16) && t.is_contiguous(),

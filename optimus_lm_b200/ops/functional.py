@@ -74,8 +74,8 @@ def gemm(a: torch.Tensor, b: torch.Tensor, M: int, N: int, K: int, *, a_mn_major
 
 def _as_2d(x: torch.Tensor) -> torch.Tensor:
     x2 = x.reshape(-1, x.shape[-1])
-    if x2.stride(-1) != 1 or (x2.stride(0) % 8) or (x2.data_ptr() % 16):
-        x2 = x2.contiguous()
+    if x2.stride(-1) != 1 or (x2.stride(0) % 8) or x2.stride(0) < x2.shape[1] or (x2.data_ptr() % 16):
+        x2 = x2.clone(memory_format=torch.contiguous_format)   # a copy: contiguous() returns misaligned rows as they are
     return x2
 
 
