@@ -81,9 +81,24 @@ struct GemmParams {
   const void* aux_in;
   long long aux_ld;
   float* aux_out;
+  // Dense mode, K range cut into k_splits parts of split_kb k-blocks each: part s writes its own partial product to rows
+  // [s * c_part_rows, + M) of C.  (Ragged-K: part = expert, c_part_rows = M.)
+  int k_splits, split_kb;
+  int c_part_rows;
+  int c_reduce;                // fp32 output added to C by the stores themselves (bulk reduction), no read in the kernel
+  const float* row_scale;      // EPI_ROWSCALE: row r of the product is multiplied by row_scale[r] before it is rounded
+  // EPI_CE: see epilogue_ce.
+  const long long* ce_targets;
+  const float* ce_ref;
+  unsigned* ce_max;
+  float* ce_part;
+  long long ce_part_ld;
+  int* ce_flags;               // [0] any row block flagged, [1 + b] row block b (128 rows) flagged
+  int ce_repair;               // only the flagged row blocks, with their rows' recorded maxima as references
+  int ce_store;                // the exponentials are written to C
 };
 
-enum { EPI_PLAIN = 0, EPI_SWIGLU = 1, EPI_SWIGLU_BWD = 2 };
+enum { EPI_PLAIN = 0, EPI_SWIGLU = 1, EPI_SWIGLU_BWD = 2, EPI_ROWSCALE = 3, EPI_CE = 4 };
 
 // All-gather fused into the GEMM: the outer rows of A live in the memories of up to 8 GPUs.  Four extra warps per
 // CTA ("stagers") copy the other GPUs' rows into this GPU's gathered copy of A with plain loads over NVLink and
@@ -161,6 +176,16 @@ struct TileInfo {
   int expert;
 };
 
+// K range of a dense or ragged-M tile: the whole of K, or part `part` of a split product.
+__device__ __forceinline__ void set_k_range(const GemmParams& p, int part, TileInfo& ti) {
+  ti.kb_begin = 0;
+  ti.kb_end = (p.K + BLOCK_K - 1) / BLOCK_K;
+  if (p.k_splits > 1) {
+    ti.kb_begin = part * p.split_kb;
+    ti.kb_end = min(ti.kb_end, ti.kb_begin + p.split_kb);
+  }
+}
+
 // Map a linear tile id to its coordinates.  Returns false when `t` is past the last tile.
 template <int BLOCK_N, int EPI = EPI_PLAIN>
 __device__ __forceinline__ bool get_tile(const GemmParams& p, int t, int num_m_blocks, int blk0, TileInfo& ti) {
@@ -178,6 +203,12 @@ __device__ __forceinline__ bool get_tile(const GemmParams& p, int t, int num_m_b
     ti.kb_end = p.meta[e + 1] / BLOCK_K;
     return true;
   }
+  int part = 0;
+  if (p.k_splits > 1) {
+    part = t / (num_m_blocks * num_n_blocks);
+    if (part >= p.k_splits) return false;
+    t -= part * (num_m_blocks * num_n_blocks);
+  }
   if (t >= num_m_blocks * num_n_blocks) return false;
   // Walk N fastest inside bands of 8 row blocks so that concurrently resident CTAs share
   // operand tiles through L2.
@@ -193,9 +224,8 @@ __device__ __forceinline__ bool get_tile(const GemmParams& p, int t, int num_m_b
   m_blk += blk0;  // first row block of the requested range
   ti.m0 = m_blk * BLOCK_M;
   ti.n0 = n_blk * TILE_N;
-  ti.kb_begin = 0;
-  ti.kb_end = (p.K + BLOCK_K - 1) / BLOCK_K;
-  ti.expert = (p.mode == OLB_GEMM_RAGGED_M) ? p.meta[1 + m_blk] : 0;
+  set_k_range(p, part, ti);
+  ti.expert = (p.mode == OLB_GEMM_RAGGED_M) ? p.meta[1 + m_blk] : part;
   return true;
 }
 
@@ -243,6 +273,7 @@ struct EpiStage {
   uint32_t base;   // shared-memory address of this warp's two buffers
   int turn;
 };
+template <bool REDUCE = false>
 __device__ __forceinline__ void epi_store_chunk(EpiStage& es, const CUtensorMap* map, const uint32_t (&v)[32], int lane,
                                                 int x, int y) {
   const uint32_t buf = es.base + (es.turn & 1) * EPI_BUF_BYTES;
@@ -256,7 +287,10 @@ __device__ __forceinline__ void epi_store_chunk(EpiStage& es, const CUtensorMap*
   fence_proxy_async_smem();
   __syncwarp();
   if (lane == 0) {
-    tma_store_2d(map, buf, x, y);
+    if (REDUCE)
+      tma_reduce_add_2d(map, buf, x, y);
+    else
+      tma_store_2d(map, buf, x, y);
     tma_store_commit();
   }
 }
@@ -264,16 +298,18 @@ __device__ __forceinline__ void epi_store_chunk(EpiStage& es, const CUtensorMap*
 // Epilogue of one 128-row accumulator tile without a fused activation: through staged tensor-map stores when the
 // output allows it, else with plain loads / stores (accumulating epilogues, layouts a tensor map cannot describe).
 // `taddr` is the accumulator's TMEM address for this warp's 32 lanes; `ti.m0` the first of the CTA's 128 rows.
-template <int BLOCK_N>
+template <int BLOCK_N, bool ROWSCALE = false>
 __device__ __forceinline__ void epilogue_plain(const GemmParams& p, const CUtensorMap* tma_c, EpiStage& es, uint32_t taddr,
                                                const TileInfo& ti, bool has_k, int lane_group, int lane) {
   const int row = ti.m0 + lane_group * 32 + lane;
   const bool row_ok = row < p.M;
+  float scale = 1.f;
+  if constexpr (ROWSCALE) scale = row_ok ? p.row_scale[row] : 0.f;
   if (p.c_tma) {
     // ---- staged tensor-map stores: 128 bytes of every row per turn (64 bf16 or 32 fp32 columns)
     long long y = ti.m0 + lane_group * 32;
     const bool rows_ok = y < p.M;
-    if (p.mode == OLB_GEMM_RAGGED_K) y += static_cast<long long>(ti.expert) * p.M;
+    y += static_cast<long long>(ti.expert) * p.c_part_rows;
     if (p.out_fp32) {
 #pragma unroll 1
       for (int c = 0; c < BLOCK_N / 32; ++c) {
@@ -286,7 +322,12 @@ __device__ __forceinline__ void epilogue_plain(const GemmParams& p, const CUtens
           for (int i = 0; i < 32; ++i) r[i] = 0u;
         }
         const int x = ti.n0 + c * 32;
-        if (rows_ok && x < p.N) epi_store_chunk(es, tma_c, r, lane, x, static_cast<int>(y));
+        if (rows_ok && x < p.N) {
+          if (p.c_reduce)
+            epi_store_chunk<true>(es, tma_c, r, lane, x, static_cast<int>(y));
+          else
+            epi_store_chunk(es, tma_c, r, lane, x, static_cast<int>(y));
+        }
       }
     } else {
 #pragma unroll 1
@@ -297,6 +338,13 @@ __device__ __forceinline__ void epilogue_plain(const GemmParams& p, const CUtens
           tmem_ld_32x32b_x32(taddr + c * 64, r0);
           tmem_ld_32x32b_x32(taddr + c * 64 + 32, r1);
           tmem_ld_wait();
+          if constexpr (ROWSCALE) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              r0[i] = __float_as_uint(scale * __uint_as_float(r0[i]));
+              r1[i] = __float_as_uint(scale * __uint_as_float(r1[i]));
+            }
+          }
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             v[i] = pack_bf16(__uint_as_float(r0[2 * i]), __uint_as_float(r0[2 * i + 1]));
@@ -485,6 +533,98 @@ __device__ __forceinline__ void epilogue_swiglu_bwd(const GemmParams& p, const C
   if (row_ok && p.aux_out) p.aux_out[static_cast<long long>(row) * ((p.N + 255) / 256) + ti.n0 / 256] = dot;
 }
 
+// Order-preserving map of a float to an unsigned (0 is below every float's image and means "none recorded").
+__device__ __forceinline__ unsigned ce_encode_max(float f) {
+  const unsigned u = __float_as_uint(f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float ce_decode_max(unsigned u) {
+  return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
+}
+// The reference that row `row`'s exponentials are taken against.
+__device__ __forceinline__ float ce_row_ref(const GemmParams& p, int row) {
+  if (p.ce_repair) {
+    const unsigned m = p.ce_max[row];
+    if (m != 0) return ce_decode_max(m);
+  }
+  return p.ce_ref[row];
+}
+// Row blocks that a repairing launch leaves alone (`blocks`: 128-row blocks per tile).
+__device__ __forceinline__ bool ce_skip_tile(const GemmParams& p, const TileInfo& ti, int blocks) {
+  if (!p.ce_repair) return false;
+  const int b = ti.m0 / BLOCK_M;
+  return p.ce_flags[1 + b] == 0 && (blocks == 1 || (b + 1) * BLOCK_M >= p.M || p.ce_flags[2 + b] == 0);
+}
+
+// Epilogue of one 128-row tile of the cross-entropy product: the accumulator holds the logits l of the row against
+// vocabulary columns [ti.n0, ti.n0 + BLOCK_N).  With the row's reference m (its target's logit, or a log-sum-exp that
+// is known already) it writes e = exp(l - m) as bf16 to C (ce_store) and the row's sum of e over the tile without
+// the target's column to ce_part[column tile][row].  exp is taken of the fp32 difference: nothing is rounded to fewer
+// bits before it, and e keeps bf16's relative precision however small it is.  Columns past N and rows without a target
+// give zeros.  A row whose logits exceed the reference by more than CE_RANGE has its largest logit recorded in ce_max
+// and its row block flagged; a second launch (ce_repair) computes those blocks again against the recorded maxima.
+// CE_RANGE: sums of 2^31 terms of e^40 = 2.4e17 stay below 1e27, far inside fp32 and bf16, and so does their inverse.
+constexpr float CE_RANGE = 40.f;
+template <int BLOCK_N>
+__device__ __forceinline__ void epilogue_ce(const GemmParams& p, const CUtensorMap* tma_c, EpiStage& es, uint32_t taddr,
+                                            const TileInfo& ti, int lane_group, int lane) {
+  const int row = ti.m0 + lane_group * 32 + lane;
+  const int y = ti.m0 + lane_group * 32;
+  if (y >= p.M) return;
+  const bool row_ok = row < p.M;
+  const long long target = row_ok ? p.ce_targets[row] : -1;
+  const bool live = target >= 0 && target < p.N;
+  const int tcol = live ? static_cast<int>(target) - ti.n0 : -1;
+  const float ref = live ? ce_row_ref(p, row) : 0.f;
+  const float2 neg_ref = make_float2(-ref, -ref);
+  const float2 log2e = make_float2(1.4426950408889634f, 1.4426950408889634f);
+  float top = -INFINITY;
+  float2 sum = make_float2(0.f, 0.f);
+#pragma unroll 1
+  for (int c = 0; c < BLOCK_N / 64; ++c) {
+    const int x = ti.n0 + c * 64;
+    if (x >= p.N) break;
+    uint32_t r[64], v[32];
+    tmem_ld_32x32b_x32(taddr + c * 64, *reinterpret_cast<uint32_t(*)[32]>(r));
+    tmem_ld_32x32b_x32(taddr + c * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(r + 32));
+    tmem_ld_wait();
+    if (x + 64 > p.N) {
+#pragma unroll
+      for (int i = 0; i < 64; ++i)
+        if (x + i >= p.N) r[i] = 0xff800000u;  // -inf: e = 0
+    }
+    const int tc = tcol - c * 64;
+    const bool here = tc >= 0 && tc < 64;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float2 l = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+      top = max3(top, l.x, l.y);
+      const float2 d = mul2(add2(l, neg_ref), log2e);
+      r[2 * i] = __float_as_uint(ex2_approx(d.x));
+      r[2 * i + 1] = __float_as_uint(ex2_approx(d.y));
+    }
+    if (__any_sync(0xffffffffu, here)) {
+#pragma unroll
+      for (int i = 0; i < 64; ++i)
+        if (i == tc) r[i] = 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float2 e = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+      sum = add2(sum, e);
+      v[i] = live ? pack_bf16(e.x, e.y) : 0u;
+    }
+    if (p.ce_store) epi_store_chunk(es, tma_c, v, lane, x, y);
+  }
+  if (!live) return;
+  if (p.ce_part) p.ce_part[static_cast<long long>(ti.n0 / BLOCK_N) * p.ce_part_ld + row] = sum.x + sum.y;
+  if (p.ce_flags && !p.ce_repair && top - ref > CE_RANGE) {
+    atomicMax(p.ce_max + row, ce_encode_max(top));
+    p.ce_flags[1 + row / BLOCK_M] = 1;
+    p.ce_flags[0] = 1;
+  }
+}
+
 // The extra warps of the variants with a fused transfer (PeerArg<true>): `swarp` is the warp's index among the CTA's
 // STAGER_WARPS stagers, `num_m_blocks` the number of 128-row blocks of the launch.
 __device__ __forceinline__ void stager_loop(const PeerArg<true>& peers, const GemmParams& p, int num_m_blocks, int swarp,
@@ -648,7 +788,11 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
   using L = SmemLayout<BLOCK_N>;
   constexpr int STAGES = L::STAGES;
   constexpr uint32_t TMEM_COLS = (2 * BLOCK_N < 32) ? 32 : 2 * BLOCK_N;
-  static_assert(EPI == EPI_PLAIN || BLOCK_N == 256, "the SwiGLU epilogue pairs 128 gate with 128 up columns");
+  static_assert(EPI != EPI_SWIGLU || BLOCK_N == 256, "the SwiGLU epilogue pairs 128 gate with 128 up columns");
+
+  if constexpr (EPI == EPI_CE) {
+    if (p.ce_repair && p.ce_flags[0] == 0) return;  // nothing to repair: the same answer in every CTA
+  }
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -708,6 +852,9 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
       bool ok = true;
       TileInfo ti;
       for (int t = blockIdx.x; ok && get_tile<BLOCK_N, EPI>(p, t, num_m_blocks, blk0, ti); t += gridDim.x) {
+        if constexpr (EPI == EPI_CE) {
+          if (ce_skip_tile(p, ti, 1)) continue;
+        }
         if constexpr (PEER) {
           // rows that the stagers bring in: wait until the whole row block is in the local operand
           bool wait_rows = false;
@@ -790,6 +937,9 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
       bool ok = true;
       TileInfo ti;
       for (int t = blockIdx.x; ok && get_tile<BLOCK_N, EPI>(p, t, num_m_blocks, blk0, ti); t += gridDim.x) {
+        if constexpr (EPI == EPI_CE) {
+          if (ce_skip_tile(p, ti, 1)) continue;
+        }
         if (ti.kb_end <= ti.kb_begin) continue;  // empty expert: the epilogue writes zeros
         if (!mbar_wait(acc_empty_bar(acc), acc_phase ^ 1u, p.status, ST_TIMEOUT_ACC_EMPTY, abort_flag)) break;
         tc_fence_after();
@@ -832,6 +982,9 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
     TileInfo ti;
     EpiStage es{smem_base + L::EPI_OFFSET + lane_group * 2 * EPI_BUF_BYTES, 0};
     for (int t = blockIdx.x; get_tile<BLOCK_N, EPI>(p, t, num_m_blocks, blk0, ti); t += gridDim.x) {
+      if constexpr (EPI == EPI_CE) {
+        if (ce_skip_tile(p, ti, 1)) continue;
+      }
       const bool has_k = ti.kb_end > ti.kb_begin;
       if (has_k) {
         if (!mbar_wait(acc_full_bar(acc), acc_phase, p.status, ST_TIMEOUT_ACC_FULL, abort_flag)) break;
@@ -842,8 +995,10 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(lane_group * 32) << 16) + acc * BLOCK_N;
       if constexpr (EPI == EPI_SWIGLU) {
         epilogue_swiglu(p, &tma_c, &tma_c2, es, taddr, ti, lane_group, lane);
+      } else if constexpr (EPI == EPI_CE) {
+        epilogue_ce<BLOCK_N>(p, &tma_c, es, taddr, ti, lane_group, lane);
       } else {
-        epilogue_plain<BLOCK_N>(p, &tma_c, es, taddr, ti, has_k, lane_group, lane);
+        epilogue_plain<BLOCK_N, EPI == EPI_ROWSCALE>(p, &tma_c, es, taddr, ti, has_k, lane_group, lane);
       }
       if constexpr (PEER) {
         if (peers.push == 1 || peers.push == 2) {  // this warp's 32 rows of the tile are stored: let the stagers know
@@ -917,6 +1072,12 @@ __device__ __forceinline__ bool get_tile_pair(const GemmParams& p, int t, int nu
     ti.kb_end = p.meta[e + 1] / BLOCK_K;
     return true;
   }
+  int part = 0;
+  if (p.k_splits > 1) {
+    part = t / (num_m * num_n);
+    if (part >= p.k_splits) return false;
+    t -= part * (num_m * num_n);
+  }
   if (t >= num_m * num_n) return false;
   constexpr int BAND = 8;
   const int band_tiles = BAND * num_n;
@@ -927,10 +1088,9 @@ __device__ __forceinline__ bool get_tile_pair(const GemmParams& p, int t, int nu
   const int m_pair = first_m + r % rows_in_band;
   ti.m0 = m_pair * 256;
   ti.n0 = (r / rows_in_band) * TILE_N;
-  ti.kb_begin = 0;
-  ti.kb_end = (p.K + BLOCK_K - 1) / BLOCK_K;
+  set_k_range(p, part, ti);
   // expert groups are padded to 256 rows (p.pair_rows), so both blocks of a pair belong to one expert
-  ti.expert = (p.mode == OLB_GEMM_RAGGED_M) ? p.meta[1 + 2 * m_pair] : 0;
+  ti.expert = (p.mode == OLB_GEMM_RAGGED_M) ? p.meta[1 + 2 * m_pair] : part;
   return true;
 }
 
@@ -944,6 +1104,10 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
   constexpr int STAGES = L::STAGES;
   constexpr int BLOCK_N = 256;
   constexpr uint32_t TMEM_COLS = 512;
+
+  if constexpr (EPI == EPI_CE) {
+    if (p.ce_repair && p.ce_flags[0] == 0) return;  // nothing to repair: the same answer in every CTA
+  }
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -1004,6 +1168,9 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
       bool ok = true;
       TileInfo ti;
       for (int t = pair_id; ok && get_tile_pair<EPI>(p, t, num_m, ti); t += num_pairs) {
+        if constexpr (EPI == EPI_CE) {
+          if (ce_skip_tile(p, ti, 2)) continue;
+        }
         const int m0 = ti.m0 + static_cast<int>(rank) * 128;
         if constexpr (PEER) {
           if (peers.push == 4) {
@@ -1085,6 +1252,9 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
       bool ok = true;
       TileInfo ti;
       for (int t = pair_id; ok && get_tile_pair<EPI>(p, t, num_m, ti); t += num_pairs) {
+        if constexpr (EPI == EPI_CE) {
+          if (ce_skip_tile(p, ti, 2)) continue;
+        }
         if (ti.kb_end <= ti.kb_begin) continue;
         if (!mbar_wait(acc_empty_bar(acc), acc_phase ^ 1u, p.status, ST_TIMEOUT_ACC_EMPTY, abort_flag)) break;
         tc_fence_after();
@@ -1129,6 +1299,9 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
     const uint32_t acc_empty_remote0 = mapa_shared(acc_empty_bar(0), 0);
     const uint32_t acc_empty_remote1 = mapa_shared(acc_empty_bar(1), 0);
     for (int t = pair_id; get_tile_pair<EPI>(p, t, num_m, ti); t += num_pairs) {
+      if constexpr (EPI == EPI_CE) {
+        if (ce_skip_tile(p, ti, 2)) continue;
+      }
       const bool has_k = ti.kb_end > ti.kb_begin;
       if (has_k) {
         if (!mbar_wait(acc_full_bar(acc), acc_phase, p.status, ST_TIMEOUT_ACC_FULL, abort_flag)) break;
@@ -1143,8 +1316,10 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
         epilogue_swiglu(p, &tma_c, &tma_c2, es, taddr, mine, lane_group, lane);
       } else if constexpr (EPI == EPI_SWIGLU_BWD) {
         epilogue_swiglu_bwd(p, &tma_c, es, taddr, mine, lane_group, lane);
+      } else if constexpr (EPI == EPI_CE) {
+        epilogue_ce<BLOCK_N>(p, &tma_c, es, taddr, mine, lane_group, lane);
       } else {
-        epilogue_plain<BLOCK_N>(p, &tma_c, es, taddr, mine, has_k, lane_group, lane);
+        epilogue_plain<BLOCK_N, EPI == EPI_ROWSCALE>(p, &tma_c, es, taddr, mine, has_k, lane_group, lane);
       }
       if constexpr (PEER) {
         if (peers.push == 1 || peers.push == 2) {  // this warp's 32 rows of the tile are stored: let the stagers know
@@ -1298,7 +1473,7 @@ static int launch(const TensorMaps& tm, const PeerArg<PEER>& peers, const GemmPa
   }
   constexpr int TILE_N = EPI == EPI_SWIGLU ? BLOCK_N / 2 : BLOCK_N;
   const long long nm = (p.M + BLOCK_M - 1) / BLOCK_M, nn = (p.N + TILE_N - 1) / TILE_N;
-  const long long tiles = nm * nn * (p.mode == OLB_GEMM_RAGGED_K ? p.num_experts : 1);
+  const long long tiles = nm * nn * (p.mode == OLB_GEMM_RAGGED_K ? p.num_experts : (p.k_splits > 1 ? p.k_splits : 1));
   int grid = static_cast<int>(tiles < num_sms ? tiles : num_sms);
   if (grid <= 0) return 0;
   gemm_bf16_kernel<BLOCK_N, PEER, EPI><<<grid, PEER ? NUM_THREADS_STAGED : NUM_THREADS, L::TOTAL, stream>>>(
@@ -1322,7 +1497,7 @@ static int launch_pair(const TensorMaps& tm, const PeerArg<PEER>& peers, const G
   }
   constexpr int TILE_N = EPI == EPI_SWIGLU ? 128 : 256;
   const long long nm = (p.M + 255) / 256, nn = (p.N + TILE_N - 1) / TILE_N;
-  const long long tiles = nm * nn * (p.mode == OLB_GEMM_RAGGED_K ? p.num_experts : 1);
+  const long long tiles = nm * nn * (p.mode == OLB_GEMM_RAGGED_K ? p.num_experts : (p.k_splits > 1 ? p.k_splits : 1));
   const int max_pairs = num_sms / 2;
   const int pairs = static_cast<int>(tiles < max_pairs ? tiles : max_pairs);
   if (pairs <= 0) return 0;
@@ -1344,6 +1519,26 @@ template <bool PEER>
 static int dispatch(int block_n, int epi, const TensorMaps& tm, const PeerArg<PEER>& peers, const GemmParams& p, int sms,
                     cudaStream_t stream) {
   if (epi == EPI_SWIGLU) return block_n == 256 ? launch<256, PEER, EPI_SWIGLU>(tm, peers, p, sms, stream) : -12;
+  if constexpr (!PEER) {
+    if (epi == EPI_ROWSCALE) {
+      switch (block_n) {
+        case 256: return launch<256, PEER, EPI_ROWSCALE>(tm, peers, p, sms, stream);
+        case 128: return launch<128, PEER, EPI_ROWSCALE>(tm, peers, p, sms, stream);
+        case 64: return launch<64, PEER, EPI_ROWSCALE>(tm, peers, p, sms, stream);
+        default: return -12;
+      }
+    }
+    if (epi == EPI_CE) {
+      switch (block_n) {
+        case 256: return launch<256, PEER, EPI_CE>(tm, peers, p, sms, stream);
+        case 128: return launch<128, PEER, EPI_CE>(tm, peers, p, sms, stream);
+        case 64: return launch<64, PEER, EPI_CE>(tm, peers, p, sms, stream);
+        default: return -12;
+      }
+    }
+  } else if (epi != EPI_PLAIN) {
+    return -14;
+  }
   switch (block_n) {
     case 256: return launch<256, PEER, EPI_PLAIN>(tm, peers, p, sms, stream);
     case 128: return launch<128, PEER, EPI_PLAIN>(tm, peers, p, sms, stream);
@@ -1363,10 +1558,18 @@ static int device_sm_count() {
 
 }  // namespace olb
 
+// Columns per statistics tile of the cross-entropy product: 256 (CTA pairs, or one CTA for fewer than 256 rows) while
+// that gives every SM work, else narrower tiles, so that a small batch still spreads the weight over the SMs.
+extern "C" int olb_gemm_ce_block_n(int M, int N) {
+  (void)M;
+  (void)N;
+  return 256;
+}
+
 extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   using namespace olb;
   if (d->M <= 0 || d->N <= 0) return 0;
-  if ((d->lda % 8) || (d->ldb % 8) || (d->ldc % 8) || (d->N % 8) || (reinterpret_cast<uintptr_t>(d->A) & 15) ||
+  if ((d->lda % 8) || (d->ldb % 8) || (d->ldc % 8) || (d->N % 8 && d->epilogue != OLB_EPI_CE) || (reinterpret_cast<uintptr_t>(d->A) & 15) ||
       (reinterpret_cast<uintptr_t>(d->B) & 15) || (reinterpret_cast<uintptr_t>(d->C) & 15))
     return -10;
   const int epi = d->epilogue;
@@ -1387,6 +1590,21 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
         ((d->row_src_of != nullptr) != (d->row_weights != nullptr)) || ((d->row_src_of != nullptr) != (d->row_k_of != nullptr)))
       return -16;
     block_n = 256;
+  } else if (epi == OLB_EPI_CE) {
+    // C = exponentials [M, N] (row stride ldc); dense, both operands K-major
+    if (d->a_mn_major || d->b_mn_major || d->accumulate || d->out_fp32 || d->mode != OLB_GEMM_DENSE || d->n_peers ||
+        d->k_split || d->k_splits > 1 || d->ce_targets == nullptr || d->ce_ref == nullptr ||
+        (d->ce_repair && (d->ce_flags == nullptr || d->ce_max == nullptr)) || (d->ce_flags != nullptr && d->ce_max == nullptr) ||
+        (d->ce_part != nullptr && d->ce_part_ld < d->M))
+      return -18;
+    block_n = olb_gemm_ce_block_n(d->M, d->N);
+  } else if (epi == OLB_EPI_ROWSCALE) {
+    if (d->row_scale == nullptr || d->accumulate || d->out_fp32 || d->mode != OLB_GEMM_DENSE || d->n_peers || d->k_splits > 1 ||
+        block_n != 0)
+      return -19;
+    block_n = d->N > 128 ? 256 : (d->N > 64 ? 128 : 64);
+  } else if (epi != OLB_EPI_PLAIN) {
+    return -12;
   } else if (block_n == 0) {
     if (d->mode != OLB_GEMM_DENSE) {
       block_n = (d->N % 256 == 0) ? 256 : (d->N % 128 == 0 ? 128 : 64);
@@ -1401,10 +1619,12 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   // (ragged-M: only when the caller padded the expert groups to 256 rows; the dense all-gather / reduce-scatter
   // variants, whose peers own multiples of 128 rows, stay on the single-CTA kernel)
   const bool pair_shape = d->block_n == 0 && block_n == 256 && d->blk_range == nullptr && d->M >= 256 && num_sms >= 2 &&
-                          (epi != OLB_EPI_PLAIN || d->N % 256 == 0 || d->N >= 2048);
+                          (epi == OLB_EPI_SWIGLU || epi == OLB_EPI_SWIGLU_BWD || epi == OLB_EPI_CE || d->N % 256 == 0 ||
+                           d->N >= 2048);
   const bool use_pair = pair_kernel_enabled() && pair_shape &&
                         (d->mode == OLB_GEMM_RAGGED_M ? (d->pair_rows != 0 && d->M % 256 == 0)
-                                                      : ((d->n_peers == 0 || d->B_peers != nullptr) && epi == OLB_EPI_PLAIN));
+                                                      : ((d->n_peers == 0 || d->B_peers != nullptr) &&
+                                                         (epi == OLB_EPI_PLAIN || epi == OLB_EPI_ROWSCALE || epi == OLB_EPI_CE)));
 
   // cuTensorMapEncodeTiled is a driver call and needs a current context in the calling thread.
   // A thread that has only been handed tensors (an autograd worker whose first CUDA work is this
@@ -1479,6 +1699,34 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   p.aux_in = d->aux_in;
   p.aux_ld = d->aux_ld;
   p.aux_out = d->aux_out;
+  p.row_scale = d->row_scale;
+  p.ce_targets = d->ce_targets;
+  p.ce_ref = d->ce_ref;
+  p.ce_max = d->ce_max;
+  p.ce_part = d->ce_part;
+  p.ce_part_ld = d->ce_part_ld;
+  p.ce_flags = d->ce_flags;
+  p.ce_repair = d->ce_repair;
+  p.ce_store = epi == OLB_EPI_CE && d->C != nullptr;
+  p.c_part_rows = d->mode == OLB_GEMM_RAGGED_K ? d->M : 0;
+  p.k_splits = 1;
+  if (d->k_splits > 1) {
+    // partial products of the K range, part s in rows [s * c_part_rows, + M) of an fp32 C; no part is empty
+    const int kb = (d->K + BLOCK_K - 1) / BLOCK_K;
+    const int per = (kb + d->k_splits - 1) / d->k_splits;
+    if (d->mode != OLB_GEMM_DENSE || epi != OLB_EPI_PLAIN || !d->out_fp32 || d->accumulate || d->n_peers || d->k_split ||
+        d->c_part_rows < d->M || d->c_part_rows % BLOCK_M || static_cast<long long>(per) * (d->k_splits - 1) >= kb)
+      return -20;
+    p.k_splits = d->k_splits;
+    p.split_kb = per;
+    p.b_expert_rows = 0;  // a part's number takes the expert's place in the tile
+    p.c_part_rows = d->c_part_rows;
+  }
+  if (d->c_reduce) {
+    if (d->mode != OLB_GEMM_DENSE || epi != OLB_EPI_PLAIN || !d->out_fp32 || d->accumulate || d->n_peers || d->k_splits > 1)
+      return -21;
+    p.c_reduce = 1;
+  }
 
   // Output through tensor-map stores whenever a 2D map describes it: no read-modify-write, and for the per-expert
   // weight gradients experts that tile exactly (a box must not run into the next expert's rows).
@@ -1494,9 +1742,15 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
     rc = make_tmap_2d(&tm.c, d->C, 2ull * d->N, d->M, d->ldc * 2, 64, 32, false);
     if (rc) return rc;
     p.c_tma = 1;
+  } else if (epi == OLB_EPI_CE) {
+    if (p.ce_store) {
+      rc = make_tmap_2d(&tm.c, d->C, d->N, d->M, d->ldc * 2, 64, 32, false);
+      if (rc) return rc;
+      p.c_tma = 1;
+    }
   } else if (!d->accumulate) {
     const uint64_t esz = d->out_fp32 ? 4 : 2;
-    uint64_t rows = d->M;
+    uint64_t rows = p.k_splits > 1 ? static_cast<uint64_t>(p.c_part_rows) * p.k_splits : d->M;
     bool ok = (d->ldc * esz) % 16 == 0;
     if (d->mode == OLB_GEMM_RAGGED_K) {
       ok = ok && d->M % BLOCK_M == 0 && d->c_expert_stride == static_cast<long long>(d->M) * d->ldc;
@@ -1508,6 +1762,7 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
       p.c_tma = 1;
     }
   }
+  if ((p.k_splits > 1 || p.c_reduce || epi == OLB_EPI_ROWSCALE) && !p.c_tma) return -22;
 
   const int sms = d->max_ctas > 0 && d->max_ctas < num_sms ? d->max_ctas : num_sms;
   if (d->n_peers > 0) {
@@ -1619,6 +1874,8 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   if (use_pair) {
     if (epi == OLB_EPI_SWIGLU) return launch_pair<false, EPI_SWIGLU>(tm, nopeers, p, sms, stream);
     if (epi == OLB_EPI_SWIGLU_BWD) return launch_pair<false, EPI_SWIGLU_BWD>(tm, nopeers, p, sms, stream);
+    if (epi == OLB_EPI_ROWSCALE) return launch_pair<false, EPI_ROWSCALE>(tm, nopeers, p, sms, stream);
+    if (epi == OLB_EPI_CE) return launch_pair<false, EPI_CE>(tm, nopeers, p, sms, stream);
     return launch_pair<false, EPI_PLAIN>(tm, nopeers, p, sms, stream);
   }
   if (epi == OLB_EPI_SWIGLU_BWD) return -16;

@@ -1,0 +1,374 @@
+// Python bindings of the cross entropy from hidden states: the launch sequences of forward and backward.
+//
+// The batch is taken in pieces of rows whose exponentials [rows, V] (bf16) fit the caller's workspace limit.
+//   one piece, gradients wanted : forward = product + finish, exponentials and row factors are kept; backward = the two
+//                                 gradient products, straight to bf16 with the incoming gradient in the row factors.
+//   several pieces, one scalar  : the incoming gradient is a common factor, so forward runs the gradient products of
+//                                 each piece too (dX to bf16, dW summed in fp32) and backward scales; every logit is
+//                                 computed once (6 T H V operations in all).
+//   several pieces, loss per row: the rows' gradients are not known in the forward, which keeps two floats per row;
+//                                 backward computes the exponentials again (8 T H V operations).
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <limits>
+
+#include "olb_api.h"
+
+namespace {
+
+inline cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+
+inline void check(int rc, const char* what) { TORCH_CHECK(rc == 0, std::string(what) + " failed with code " + std::to_string(rc)); }
+
+enum { MEAN = 0, SUM = 1, NONE = 2 };
+
+int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+
+struct Problem {
+  at::Tensor x, w, targets;
+  int64_t T, H, V, lde;
+  int* status;
+  cudaStream_t stream;
+};
+
+Problem make_problem(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, const at::Tensor& status) {
+  TORCH_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16 && x.dim() == 2 && x.stride(1) == 1, "x must be a 2D CUDA bf16 tensor with unit inner stride");
+  TORCH_CHECK(w.is_cuda() && w.scalar_type() == at::kBFloat16 && w.dim() == 2 && w.stride(1) == 1, "weight must be a 2D CUDA bf16 tensor with unit inner stride");
+  TORCH_CHECK(targets.is_cuda() && targets.scalar_type() == at::kLong && targets.dim() == 1 && targets.is_contiguous(), "targets must be a contiguous 1D CUDA int64 tensor");
+  TORCH_CHECK(x.device() == w.device() && x.device() == targets.device() && x.device() == status.device(), "x, weight, targets must be on one device");
+  TORCH_CHECK(x.size(1) == w.size(1) && x.size(0) == targets.size(0), "shapes of x, weight, targets do not match");
+  TORCH_CHECK(x.size(1) % 8 == 0 && x.size(1) > 0 && w.size(0) > 0, "the hidden size must be a positive multiple of 8");
+  TORCH_CHECK(x.size(0) < (1ll << 31) - 256 && w.size(0) < (1ll << 31) - 256 && w.size(1) < (1ll << 31), "too many rows");
+  return {x, w, targets, x.size(0), x.size(1), w.size(0), round_up(w.size(0), 64), status.data_ptr<int>(), cur_stream()};
+}
+
+int64_t piece_rows(int64_t T, int64_t bytes_per_row, int64_t max_bytes) {
+  const int64_t most = std::max<int64_t>(256, max_bytes / bytes_per_row / 256 * 256);
+  const int64_t n = std::max<int64_t>(1, (T + most - 1) / most);
+  return n == 1 ? T : round_up((T + n - 1) / n, 256);
+}
+
+const long long* ptr_i64(const at::Tensor& t, int64_t at) { return reinterpret_cast<const long long*>(t.data_ptr<int64_t>()) + at; }
+void* row_ptr(const at::Tensor& t, int64_t row) { return static_cast<char*>(t.data_ptr()) + row * t.stride(0) * t.element_size(); }
+
+// Parts of the K range for C [M, N] += A [M, K] B: enough that the tiles fill the SMs, as few as possible.  Costs in
+// microseconds: a k-block of a tile at 1.5 PFLOP/s over the GPU, whole waves of tiles, and for more than one part the
+// fp32 partial products written and read once at 4.5 TB/s plus the launch that sums them.
+int split_parts(int64_t M, int64_t N, int64_t K) {
+  int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  const bool pair = M >= 256 && (N % 256 == 0 || N >= 2048);
+  const int64_t tm = pair ? 256 : 128, tn = N > 128 ? 256 : (N > 64 ? 128 : 64), workers = pair ? sms / 2 : sms;
+  const int64_t tiles = ((M + tm - 1) / tm) * ((N + tn - 1) / tn), kb = (K + 63) / 64;
+  const double block_us = 2.0 * tm * tn * 64 * workers / 1.5e9;
+  int best = 1;
+  double least = 1e30;
+  for (int s = 1; s <= 64 && (s == 1 || kb / s >= 8); ++s) {
+    const int64_t per = (kb + s - 1) / s;
+    if (per * (s - 1) >= kb) continue;
+    const double cost = ((tiles * s + workers - 1) / workers) * per * block_us + (s > 1 ? 8.0 * s * M * N / 4.5e6 + 4.0 : 0.0);
+    if (cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
+// e = exp(l - ref) of one piece (and the sums of its tiles), then the row blocks that need another reference.
+void product(const Problem& p, int64_t r0, int64_t rows, const float* ref, unsigned* top, int* flags, float* part,
+             int64_t part_ld, void* E) {
+  olb_gemm_desc d{};
+  d.A = row_ptr(p.x, r0);
+  d.B = p.w.data_ptr();
+  d.C = E;
+  d.lda = p.x.stride(0);
+  d.ldb = p.w.stride(0);
+  d.ldc = p.lde;
+  d.a_rows = rows;
+  d.b_rows = p.V;
+  d.M = static_cast<int>(rows);
+  d.N = static_cast<int>(p.V);
+  d.K = static_cast<int>(p.H);
+  d.epilogue = OLB_EPI_CE;
+  d.status = p.status;
+  d.ce_targets = ptr_i64(p.targets, r0);
+  d.ce_ref = ref;
+  d.ce_max = top;
+  d.ce_flags = flags;
+  d.ce_part = part;
+  d.ce_part_ld = part_ld;
+  check(olb_gemm_bf16(&d, p.stream), "olb_gemm_bf16 (cross entropy)");
+  if (flags) {
+    d.ce_repair = 1;
+    check(olb_gemm_bf16(&d, p.stream), "olb_gemm_bf16 (cross entropy, repair)");
+  }
+}
+
+// dx[r0 .. r0 + rows) = row_factor * (E W)
+void input_gradient(const Problem& p, int64_t r0, int64_t rows, const void* E, const float* row_factor, at::Tensor& dx) {
+  const int parts = split_parts(rows, p.H, p.V);
+  olb_gemm_desc d{};
+  d.A = E;
+  d.B = p.w.data_ptr();
+  d.lda = p.lde;
+  d.ldb = p.w.stride(0);
+  d.a_rows = rows;
+  d.b_rows = p.V;
+  d.M = static_cast<int>(rows);
+  d.N = static_cast<int>(p.H);
+  d.K = static_cast<int>(p.V);
+  d.b_mn_major = 1;
+  d.status = p.status;
+  d.ldc = p.H;
+  if (parts == 1) {
+    d.epilogue = OLB_EPI_ROWSCALE;
+    d.row_scale = row_factor;
+    d.C = row_ptr(dx, r0);
+    check(olb_gemm_bf16(&d, p.stream), "olb_gemm_bf16 (input gradient)");
+    return;
+  }
+  const int64_t part_rows = round_up(rows, 128);
+  at::Tensor partial = at::empty({parts * part_rows, p.H}, p.x.options().dtype(at::kFloat));
+  d.C = partial.data_ptr();
+  d.out_fp32 = 1;
+  d.k_splits = parts;
+  d.c_part_rows = static_cast<int>(part_rows);
+  check(olb_gemm_bf16(&d, p.stream), "olb_gemm_bf16 (input gradient)");
+  check(olb_lce_sum_parts(partial.data_ptr<float>(), parts, part_rows, static_cast<int>(rows), static_cast<int>(p.H),
+                          row_factor, row_ptr(dx, r0), p.stream),
+        "olb_lce_sum_parts");
+}
+
+// dw (=, += or, in fp32, reduced into) E^T xs
+void weight_gradient(const Problem& p, int64_t rows, const void* E, const void* xs, at::Tensor& dw, bool add) {
+  olb_gemm_desc d{};
+  d.A = E;
+  d.B = xs;
+  d.C = dw.data_ptr();
+  d.lda = p.lde;
+  d.ldb = p.H;
+  d.ldc = dw.stride(0);
+  d.a_rows = rows;
+  d.b_rows = rows;
+  d.M = static_cast<int>(p.V);
+  d.N = static_cast<int>(p.H);
+  d.K = static_cast<int>(rows);
+  d.a_mn_major = d.b_mn_major = 1;
+  d.status = p.status;
+  d.out_fp32 = dw.scalar_type() == at::kFloat;
+  if (d.out_fp32)
+    d.c_reduce = add;
+  else
+    d.accumulate = add;
+  check(olb_gemm_bf16(&d, p.stream), "olb_gemm_bf16 (weight gradient)");
+}
+
+at::Tensor weight_gradient_out(const Problem& p, const c10::optional<at::Tensor>& dw_out, bool accumulate) {
+  if (!dw_out.has_value()) {
+    TORCH_CHECK(!accumulate, "nothing to accumulate into");
+    return at::empty({p.V, p.H}, p.w.options());
+  }
+  TORCH_CHECK(dw_out->scalar_type() == at::kBFloat16 && dw_out->device() == p.w.device() && dw_out->is_contiguous() &&
+              dw_out->dim() == 2 && dw_out->size(0) == p.V && dw_out->size(1) == p.H, "dw_out must be a contiguous bf16 [V, H] tensor");
+  return *dw_out;
+}
+
+// Returns the loss (a scalar, or [T] for NONE) and what the backward needs: with one piece {E, factor}; with several
+// {dx, dw32} for a scalar loss (undefined where not wanted), {prob, lse} for losses per row.
+std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, int64_t reduction,
+                                      bool need_dx, bool need_dw, int64_t max_bytes, const at::Tensor& status) {
+  TORCH_CHECK(reduction >= MEAN && reduction <= NONE);
+  c10::cuda::CUDAGuard guard(x.device());
+  const Problem p = make_problem(x, w, targets, status);
+  const bool grad = need_dx || need_dw;
+  const auto f32 = x.options().dtype(at::kFloat);
+  if (p.T == 0) {
+    at::Tensor out = reduction == NONE ? at::empty({0}, f32)
+                                       : at::full({}, reduction == MEAN ? std::numeric_limits<double>::quiet_NaN() : 0.0, f32);
+    return {out, at::empty({0, p.lde}, x.options()), at::empty({0}, f32)};
+  }
+  const int64_t tile = olb_gemm_ce_block_n(static_cast<int>(p.T), static_cast<int>(p.V));
+  int64_t rows_max = piece_rows(p.T, grad ? 2 * p.lde : 4 * ((p.V + 63) / 64), max_bytes);
+  const bool single = rows_max >= p.T;
+  const bool store = grad && (single || reduction != NONE);   // several pieces of losses per row: exponentials again later
+  if (grad && !single && reduction == NONE) rows_max = piece_rows(p.T, 4 * ((p.V + 63) / 64), max_bytes);
+  const int64_t ntiles_most = (p.V + 63) / 64;
+  (void)tile;
+
+  at::Tensor loss_rows = at::empty({p.T}, f32);
+  at::Tensor out = reduction == NONE ? loss_rows : at::empty({}, f32);
+  // small per-row and per-launch words: ref, top, flags, ticket, count, 1 / count
+  at::Tensor words = at::empty({2 * rows_max + (rows_max + 127) / 128 + 1 + 3}, f32);
+  float* ref = words.data_ptr<float>();
+  unsigned* top = reinterpret_cast<unsigned*>(ref + rows_max);
+  int* flags = reinterpret_cast<int*>(top + rows_max);
+  unsigned* ticket = reinterpret_cast<unsigned*>(flags + (rows_max + 127) / 128 + 1);
+  float* count = reinterpret_cast<float*>(ticket + 1);
+  at::Tensor part = at::empty({ntiles_most, rows_max}, f32);
+  at::Tensor E, factor, dx, dw32, prob, lse, xs;
+  if (store) {
+    E = at::empty({rows_max, p.lde}, x.options());
+    factor = at::empty({rows_max}, f32);
+  }
+  const bool in_forward = store && !single;
+  if (in_forward) {
+    if (need_dx) dx = at::empty({p.T, p.H}, x.options());
+    if (need_dw) {
+      dw32 = at::empty({p.V, p.H}, f32);
+      xs = at::empty({rows_max, p.H}, x.options());
+    }
+  }
+  if (grad && !store) {
+    prob = at::empty({p.T}, f32);
+    lse = at::empty({p.T}, f32);
+  }
+  if (reduction == MEAN)
+    check(olb_lce_count(ptr_i64(p.targets, 0), p.T, static_cast<int>(p.V), count, count + 1, p.stream), "olb_lce_count");
+  for (int64_t r0 = 0; r0 < p.T; r0 += rows_max) {
+    const int64_t rows = std::min(rows_max, p.T - r0);
+    const int bn = olb_gemm_ce_block_n(static_cast<int>(rows), static_cast<int>(p.V));
+    check(olb_lce_prep(row_ptr(x, r0), x.stride(0), w.data_ptr(), w.stride(0), ptr_i64(p.targets, r0), static_cast<int>(rows),
+                       static_cast<int>(p.H), static_cast<int>(p.V), ref, top, flags, ticket, p.stream),
+          "olb_lce_prep");
+    product(p, r0, rows, ref, top, flags, part.data_ptr<float>(), rows_max, store ? E.data_ptr() : nullptr);
+    olb_lce_finish_desc f{};
+    f.part = part.data_ptr<float>();
+    f.part_ld = rows_max;
+    f.ntiles = static_cast<int>((p.V + bn - 1) / bn);
+    f.ref = ref;
+    f.ce_max = top;
+    f.targets = ptr_i64(p.targets, r0);
+    f.rows = static_cast<int>(rows);
+    f.V = static_cast<int>(p.V);
+    f.H = static_cast<int>(p.H);
+    f.loss = loss_rows.data_ptr<float>() + r0;
+    if (prob.defined()) {
+      f.prob = prob.data_ptr<float>() + r0;
+      f.lse = lse.data_ptr<float>() + r0;
+    }
+    if (store) {
+      f.E = E.data_ptr();
+      f.lde = p.lde;
+      f.factor = factor.data_ptr<float>();
+      f.scale = reduction == MEAN ? count + 1 : nullptr;
+    }
+    if (xs.defined()) {
+      f.x = row_ptr(x, r0);
+      f.ldx = x.stride(0);
+      f.xs = xs.data_ptr();
+    }
+    if (reduction != NONE && r0 + rows == p.T) {
+      f.ticket = ticket;
+      f.loss_all = loss_rows.data_ptr<float>();
+      f.n_all = p.T;
+      f.total = out.data_ptr<float>();
+      f.total_scale = reduction == MEAN ? count : nullptr;
+    }
+    check(olb_lce_finish(&f, p.stream), "olb_lce_finish");
+    if (in_forward) {
+      if (need_dx) input_gradient(p, r0, rows, E.data_ptr(), factor.data_ptr<float>(), dx);
+      if (need_dw) weight_gradient(p, rows, E.data_ptr(), xs.data_ptr(), dw32, r0 > 0);
+    }
+  }
+  if (!grad) return {out};
+  if (in_forward) return {out, dx, dw32};
+  if (store) return {out, E, factor};
+  return {out, prob, lse};
+}
+
+// One piece: E and factor as the forward left them; grad is a scalar or [T].  Returns {dx, dw} (undefined where not
+// wanted; dw is dw_out when that is given).
+std::vector<at::Tensor> linear_ce_bwd(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, const at::Tensor& E,
+                                      const at::Tensor& factor, const at::Tensor& grad, bool need_dx, bool need_dw,
+                                      const c10::optional<at::Tensor>& dw_out, bool accumulate, const at::Tensor& status) {
+  c10::cuda::CUDAGuard guard(x.device());
+  const Problem p = make_problem(x, w, targets, status);
+  TORCH_CHECK(grad.scalar_type() == at::kFloat && grad.device() == x.device() && grad.is_contiguous() &&
+              (grad.numel() == 1 || grad.numel() == p.T), "grad must be one fp32 value or one for each row");
+  TORCH_CHECK(E.scalar_type() == at::kBFloat16 && E.size(0) >= p.T && E.size(1) == p.lde && E.is_contiguous() && factor.numel() >= p.T);
+  at::Tensor dx, dw;
+  if (need_dx) dx = at::empty({p.T, p.H}, x.options());
+  if (need_dw) dw = weight_gradient_out(p, dw_out, accumulate);
+  if (p.T == 0) {
+    if (need_dw && !accumulate) dw.zero_();
+    return {dx, dw};
+  }
+  at::Tensor row_factor = at::empty({p.T}, x.options().dtype(at::kFloat));
+  at::Tensor xs = need_dw ? at::empty({p.T, p.H}, x.options()) : at::Tensor();
+  check(olb_lce_scale_rows(x.data_ptr(), x.stride(0), factor.data_ptr<float>(), grad.data_ptr<float>(),
+                           grad.dim() == 0 ? 0 : 1, static_cast<int>(p.T), static_cast<int>(p.H), row_factor.data_ptr<float>(),
+                           need_dw ? xs.data_ptr() : nullptr, p.stream),
+        "olb_lce_scale_rows");
+  if (need_dx) input_gradient(p, 0, p.T, E.data_ptr(), row_factor.data_ptr<float>(), dx);
+  if (need_dw) weight_gradient(p, p.T, E.data_ptr(), xs.data_ptr(), dw, accumulate);
+  return {dx, dw};
+}
+
+// Several pieces of a scalar loss: the gradients of the forward times the incoming gradient.
+std::vector<at::Tensor> linear_ce_bwd_scale(const c10::optional<at::Tensor>& dx_in, const c10::optional<at::Tensor>& dw32,
+                                            const at::Tensor& grad, const c10::optional<at::Tensor>& dw_out, bool accumulate) {
+  const at::Tensor& any = dx_in.has_value() ? *dx_in : *dw32;
+  c10::cuda::CUDAGuard guard(any.device());
+  TORCH_CHECK(grad.scalar_type() == at::kFloat && grad.numel() == 1 && grad.device() == any.device());
+  at::Tensor dx, dw;
+  if (dx_in.has_value()) {
+    dx = at::empty_like(*dx_in);
+    check(olb_lce_scale_out(dx_in->data_ptr(), 1, dx.numel(), grad.data_ptr<float>(), dx.data_ptr(), 0, cur_stream()), "olb_lce_scale_out");
+  }
+  if (dw32.has_value()) {
+    TORCH_CHECK(!accumulate || dw_out.has_value());
+    dw = dw_out.has_value() ? *dw_out : at::empty(dw32->sizes(), dw32->options().dtype(at::kBFloat16));
+    TORCH_CHECK(dw.scalar_type() == at::kBFloat16 && dw.is_contiguous() && dw.sizes() == dw32->sizes() && dw.device() == dw32->device());
+    check(olb_lce_scale_out(dw32->data_ptr(), 0, dw.numel(), grad.data_ptr<float>(), dw.data_ptr(), accumulate, cur_stream()), "olb_lce_scale_out");
+  }
+  return {dx, dw};
+}
+
+// Several pieces of losses per row: exponentials against the known log-sum-exp, piece by piece.
+std::vector<at::Tensor> linear_ce_bwd_again(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets,
+                                            const at::Tensor& prob, const at::Tensor& lse, const at::Tensor& grad, bool need_dx,
+                                            bool need_dw, int64_t max_bytes, const c10::optional<at::Tensor>& dw_out,
+                                            bool accumulate, const at::Tensor& status) {
+  c10::cuda::CUDAGuard guard(x.device());
+  const Problem p = make_problem(x, w, targets, status);
+  TORCH_CHECK(grad.scalar_type() == at::kFloat && grad.device() == x.device() && grad.is_contiguous() && grad.numel() == p.T &&
+              prob.numel() == p.T && lse.numel() == p.T);
+  const auto f32 = x.options().dtype(at::kFloat);
+  const int64_t rows_max = piece_rows(p.T, 2 * p.lde, max_bytes);
+  at::Tensor E = at::empty({rows_max, p.lde}, x.options());
+  at::Tensor factor = at::empty({rows_max}, f32), row_factor = at::empty({rows_max}, f32);
+  at::Tensor dx, dw, dw32, xs;
+  if (need_dx) dx = at::empty({p.T, p.H}, x.options());
+  if (need_dw) {
+    dw = weight_gradient_out(p, dw_out, accumulate);
+    dw32 = at::empty({p.V, p.H}, f32);
+    xs = at::empty({rows_max, p.H}, x.options());
+  }
+  for (int64_t r0 = 0; r0 < p.T; r0 += rows_max) {
+    const int64_t rows = std::min(rows_max, p.T - r0);
+    product(p, r0, rows, lse.data_ptr<float>() + r0, nullptr, nullptr, nullptr, 0, E.data_ptr());
+    check(olb_lce_patch(prob.data_ptr<float>() + r0, ptr_i64(p.targets, r0), static_cast<int>(rows), static_cast<int>(p.V),
+                        E.data_ptr(), p.lde, factor.data_ptr<float>(), p.stream),
+          "olb_lce_patch");
+    check(olb_lce_scale_rows(row_ptr(x, r0), x.stride(0), factor.data_ptr<float>(), grad.data_ptr<float>() + r0, 1,
+                             static_cast<int>(rows), static_cast<int>(p.H), row_factor.data_ptr<float>(),
+                             need_dw ? xs.data_ptr() : nullptr, p.stream),
+          "olb_lce_scale_rows");
+    if (need_dx) input_gradient(p, r0, rows, E.data_ptr(), row_factor.data_ptr<float>(), dx);
+    if (need_dw) weight_gradient(p, rows, E.data_ptr(), xs.data_ptr(), dw32, r0 > 0);
+  }
+  if (need_dw)
+    check(olb_lce_scale_out(dw32.data_ptr(), 0, dw32.numel(), nullptr, dw.data_ptr(), accumulate, p.stream), "olb_lce_scale_out");
+  return {dx, dw};
+}
+
+}  // namespace
+
+void register_linear_ce(pybind11::module& m) {
+  m.def("linear_ce_fwd", &linear_ce_fwd);
+  m.def("linear_ce_bwd", &linear_ce_bwd);
+  m.def("linear_ce_bwd_scale", &linear_ce_bwd_scale);
+  m.def("linear_ce_bwd_again", &linear_ce_bwd_again);
+}

@@ -11,7 +11,7 @@ extern "C" {
 
 // ---------------------------------------------------------------- GEMM (gemm_tcgen05.cu)
 enum { OLB_GEMM_DENSE = 0, OLB_GEMM_RAGGED_M = 1, OLB_GEMM_RAGGED_K = 2 };
-enum { OLB_EPI_PLAIN = 0, OLB_EPI_SWIGLU = 1, OLB_EPI_SWIGLU_BWD = 2 };
+enum { OLB_EPI_PLAIN = 0, OLB_EPI_SWIGLU = 1, OLB_EPI_SWIGLU_BWD = 2, OLB_EPI_ROWSCALE = 3, OLB_EPI_CE = 4 };
 
 typedef struct {
   const void* A;  // bf16. K-major: [a_rows, K] with row stride lda; MN-major: [a_rows (=K extent), M]
@@ -93,9 +93,29 @@ typedef struct {
   // (one int per 128 rows of B, zero at launch) counts the 16-byte vectors landed.  B is complete when the launch ends.
   const void* const* B_peers;
   const long long* b_seg;    // host array [2 * n_peers]
+  // Split K (DENSE, fp32 C): k_splits > 1 parts of whole 64-element blocks, none of them empty; part s is written to rows
+  // [s * c_part_rows, + M) of C (c_part_rows >= M, a multiple of 128), to be summed by the caller.
+  int k_splits, c_part_rows;
+  int c_reduce;              // DENSE, fp32 C: C += A*B through reducing bulk stores (the kernel does not read C)
+  const float* row_scale;    // epilogue == OLB_EPI_ROWSCALE (DENSE, bf16 C): row r of the product times row_scale[r]
+  // Cross-entropy product (epilogue == OLB_EPI_CE; DENSE, K-major operands): A = hidden states, B = the head's weight
+  // [N, K] with any number of rows N.  Row r has its target in ce_targets[r] (outside [0, N): no target) and a reference
+  // ce_ref[r]; with l the logits, C (may be NULL) receives exp(l - ref) as bf16, zeros for rows without a target, and
+  // ce_part[tile * ce_part_ld + r] (may be NULL) the sum of exp(l - ref) over column tile `tile` (olb_gemm_ce_block_n
+  // columns each) without the target's column.  ce_flags (may be NULL; 1 + ceil(M / 128) ints and ce_max M words, all
+  // zero): a row whose largest logit exceeds its reference by more than 40 has it recorded in ce_max and its block of
+  // 128 rows flagged.  ce_repair: the same product for the flagged blocks alone, rows with a recorded maximum against that.
+  const long long* ce_targets;
+  const float* ce_ref;
+  unsigned* ce_max;
+  float* ce_part;
+  long long ce_part_ld;
+  int* ce_flags;
+  int ce_repair;
 } olb_gemm_desc;
 
 int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream);
+int olb_gemm_ce_block_n(int M, int N);
 
 // ---------------------------------------------------------------- normalisation (norm.cu)
 // y = x * rsqrt(mean(x^2) + eps) * w   (w may be NULL).  rstd [rows] fp32 is saved for backward.
@@ -209,6 +229,55 @@ int olb_ce_partial_fwd(const void* logits, long long ldl, const long long* label
                        float* part_sum, float* part_tgt, int rows, int V, cudaStream_t stream);
 int olb_ce_partial_bwd(const void* logits, long long ldl, const long long* labels, int v_start, int v_total,
                        const float* lse, const float* scale_dev, void* dlogits, int rows, int V, cudaStream_t stream);
+
+// ---------------------------------------------------------------- cross entropy from hidden states (linear_ce.cu)
+// The passes around the OLB_EPI_CE product; `rows` is one piece of the batch (see linear_ce.cu for the formulas).
+// ref[r] = x_r . w_t (fp32) for rows with a target t in [0, V), else 0; zeroes ce_max [rows], ce_flags
+// [1 + ceil(rows / 128)] and *ticket.
+int olb_lce_prep(const void* x, long long ldx, const void* w, long long ldw, const long long* targets, int rows, int H,
+                 int V, float* ref, unsigned* ce_max, int* ce_flags, unsigned* ticket, cudaStream_t stream);
+// *count = number of targets in [0, V) (as fp32; exact up to 2^24), *inv_count = 1 / *count (0 when there are none).
+int olb_lce_count(const long long* targets, long long n, int V, float* count, float* inv_count, cudaStream_t stream);
+// Sums ce_part over its `ntiles` tiles and writes per row loss[r] (0 without a target) and, when they are not NULL,
+// prob[r] = 1 - p_target, lse[r], and with E (the exponentials, row stride lde): the target's entry of E, and
+// factor[r] such that factor[r] * E[r, :] is the row's gradient (times *scale when scale is not NULL); xs (may be NULL):
+// bf16(factor[r] * x[r, :]).  total (may be NULL): sum of loss_all[0, n_all) times *total_scale (NULL: 1), taken by
+// the last block through *ticket.
+typedef struct {
+  const float* part;
+  long long part_ld;
+  int ntiles;
+  const float* ref;
+  const unsigned* ce_max;
+  const long long* targets;
+  int rows, V, H;
+  float *loss, *prob, *lse, *factor;
+  void* E;
+  long long lde;
+  const float* scale;
+  const void* x;
+  long long ldx;
+  void* xs;
+  unsigned* ticket;
+  const float* loss_all;
+  long long n_all;
+  const float* total_scale;
+  float* total;
+} olb_lce_finish_desc;
+int olb_lce_finish(const olb_lce_finish_desc* d, cudaStream_t stream);
+// The target entries of exponentials that were taken against the log-sum-exp: E[r, t] = -prob[r] (rounded), factor[r]
+// as above with the row's gradient grad[r * grad_stride].
+int olb_lce_patch(const float* prob, const long long* targets, int rows, int V, void* E, long long lde, float* factor,
+                  cudaStream_t stream);
+// row_factor[r] = factor[r] * grad[r * grad_stride] and, when xs is not NULL, xs[r, :] = bf16(row_factor[r] * x[r, :]).
+int olb_lce_scale_rows(const void* x, long long ldx, const float* factor, const float* grad, long long grad_stride, int rows,
+                       int H, float* row_factor, void* xs, cudaStream_t stream);
+// out[r, :] = bf16(row_factor[r] * sum_s part[s * part_rows + r, :]) in the order of s.
+int olb_lce_sum_parts(const float* part, int nparts, long long part_rows, int rows, int H, const float* row_factor, void* out,
+                      cudaStream_t stream);
+// dst (bf16) = (accumulate ? dst : 0) + *grad * src (NULL: 1), src fp32 or (src_bf16) bf16, n elements.
+int olb_lce_scale_out(const void* src, int src_bf16, long long n, const float* grad, void* dst, int accumulate,
+                      cudaStream_t stream);
 
 // ---------------------------------------------------------------- optimizer (adamw.cu)
 typedef struct {
