@@ -440,6 +440,7 @@ void register_attention(pybind11::module& m);
 void register_comm(pybind11::module& m);
 void register_customops(pybind11::module& m);
 void register_linear_ce(pybind11::module& m);
+void register_grad_clip(pybind11::module& m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm", &gemm, pybind11::arg("a"), pybind11::arg("b"), pybind11::arg("c"), pybind11::arg("M"), pybind11::arg("N"),
@@ -488,4 +489,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_comm(m);
   register_customops(m);
   register_linear_ce(m);
+  register_grad_clip(m);
 }

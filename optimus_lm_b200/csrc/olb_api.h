@@ -301,6 +301,19 @@ int olb_adamw_step(const void* grad, int grad_fp32, float* master, float* m, flo
                    long long n, const olb_adamw_hparams* hp, const float* clip_coef_dev, float* norm_partial,
                    cudaStream_t stream);
 
+// ---------------------------------------------------------------- gradient norm over a list (grad_clip.cu)
+typedef struct {
+  void* ptr;       // device memory, aligned to its element type
+  long long n;     // elements
+  int fp32;        // 0: bf16
+} olb_clip_tensor;
+// *norm_out = sqrt(sum of squares), or the largest absolute value (inf_norm), over the n tensors of the host array
+// `list`; with `scale` they are multiplied in place by min(1, max_norm / (norm + eps)).  partial: scratch of
+// `room` >= olb_grad_clip_parts(list, n) doubles.  The tensors must not overlap when they are scaled.
+int olb_grad_clip(const olb_clip_tensor* list, int n, int inf_norm, int scale, float max_norm, float eps, double* partial,
+                  int room, float* norm_out, cudaStream_t stream);
+int olb_grad_clip_parts(const olb_clip_tensor* list, int n);
+
 // ---------------------------------------------------------------- reference custom-op interface (customops.cu)
 // The seven entry points of the reference's pcl_xpu_customops extension on its data layout (see customops.cu).
 // int32 indices; data bf16, or fp32 when `fp32` is set.

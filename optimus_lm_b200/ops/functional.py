@@ -1185,3 +1185,60 @@ def sum_of_squares(t: torch.Tensor, scale: float = 1.0, out: Optional[torch.Tens
         else:
             out.copy_(s)
     return out
+
+
+def _grad_norm_reference(grads, norm_type):
+    if norm_type == math.inf:
+        return torch.stack([g.detach().abs().max().float() for g in grads]).max()
+    return torch.stack([g.detach().double().square().sum() for g in grads]).sum().sqrt().float()
+
+
+def _check_grads(grads, norm_type):
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    if norm_type not in (2, math.inf):
+        raise ValueError(f"norm_type must be 2 or inf, not {norm_type!r}")
+    return grads
+
+
+def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
+    """Norm of all elements of the tensors ``grads`` together (Euclidean, or the largest absolute value with
+    ``norm_type=inf``) as a 0-dim fp32 tensor on their device.
+
+    One call for any number of tensors, of any length and alignment (two launches up to 2040 tensors), bf16 and fp32 mixed;
+    squares are summed in fp64 beyond 16 bytes, so that neither their number nor their size shows, and the bits are
+    the same every run.  Other types and CPU tensors take the plain path.  All tensors must be on one device.
+    Reference: ``torch.nn.utils.get_total_norm`` on the parameters' gradients (dist_train.py:889-906)."""
+    grads = _check_grads(grads, norm_type)
+    if not grads:
+        return torch.zeros(())
+    if use_kernels(grads[0]):
+        norm = extension().grad_clip(grads, norm_type == math.inf, False, 0.0, 0.0)
+        if norm is not None:
+            return norm
+    if any(g.device != grads[0].device for g in grads):
+        raise ValueError("the gradients are on different devices")
+    grads = [g for g in grads if g.numel()]
+    return _grad_norm_reference(grads, norm_type) if grads else torch.zeros(())
+
+
+@torch.no_grad()
+def clip_grad_norm_(grads, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
+    """Scale the tensors ``grads`` in place by ``min(1, max_norm / (norm + 1e-6))`` and return ``norm`` (see
+    ``grad_norm``) as it was before.  The factor stays on the device: no synchronisation, and the call can be captured
+    into a graph.  Gradients that need no scaling are read once and not written.  A norm that is not finite makes
+    the factor 0 or NaN, which reaches the gradients.  The tensors must not share memory."""
+    grads = _check_grads(grads, norm_type)
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm must not be negative: {max_norm}")
+    if not grads:
+        return torch.zeros(())
+    if use_kernels(grads[0]):
+        norm = extension().grad_clip(grads, norm_type == math.inf, True, max_norm, 1e-6)
+        if norm is not None:
+            return norm
+    norm = grad_norm(grads, norm_type)
+    factor = torch.clamp(max_norm / (norm + 1e-6), max=1.0)
+    for g in grads:
+        g.copy_(g.float() * factor if g.dtype != torch.float64 else g * factor)
+    return norm

@@ -1,0 +1,45 @@
+"""Gradient norm and clipping on the plain path, and what the calls refuse."""
+import math
+
+import pytest
+import torch
+
+from optimus_lm_b200.ops import functional as OF
+
+
+@pytest.mark.parametrize("norm_type", [2.0, math.inf])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
+def test_plain_path(norm_type, dtype):
+    g = torch.Generator().manual_seed(0)
+    grads = [torch.randn(5, 7, generator=g).to(dtype), torch.randn(0).to(dtype), torch.randn(11, generator=g).to(dtype)[::2]]
+    before = [x.clone() for x in grads]
+    want = torch.linalg.vector_norm(torch.cat([x.double().reshape(-1) for x in grads]), norm_type)
+    assert torch.allclose(OF.grad_norm(grads, norm_type).double(), want, rtol=1e-6)
+    norm = OF.clip_grad_norm_(grads, 0.5, norm_type)
+    assert norm.dtype == torch.float32 and torch.allclose(norm.double(), want, rtol=1e-6)
+    for a, b in zip(grads, before):
+        assert torch.allclose(a.double(), b.double() * (0.5 / (want + 1e-6)), rtol=2.0 ** -8 if dtype == torch.bfloat16 else 1e-6)
+    again = [x.clone() for x in grads]
+    OF.clip_grad_norm_(iter(grads), 100.0, norm_type)
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
+
+
+def test_single_tensor_and_empty():
+    assert OF.grad_norm(torch.tensor([3.0, 4.0])).item() == 5
+    assert OF.grad_norm([]).item() == 0 and OF.clip_grad_norm_([], 1.0).item() == 0
+    assert OF.grad_norm([torch.zeros(0)]).item() == 0 and OF.clip_grad_norm_([torch.zeros(0)], 1.0).item() == 0
+
+
+def test_refusals():
+    g = [torch.ones(3)]
+    for bad in (1, 3.0, -math.inf, "fro"):
+        with pytest.raises(ValueError):
+            OF.grad_norm(g, bad)
+        with pytest.raises(ValueError):
+            OF.clip_grad_norm_(g, 1.0, bad)
+    for bad in (-1.0, math.nan):
+        with pytest.raises(ValueError):
+            OF.clip_grad_norm_(g, bad)
+    with pytest.raises(ValueError):
+        OF.grad_norm([torch.ones(3), torch.ones(3, device="meta")])
+    assert torch.equal(g[0], torch.ones(3))
