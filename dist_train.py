@@ -139,6 +139,11 @@ def build_parser():
     p.add_argument("--disable_fused_ep_alltoall", action="store_true", help="Use the NCCL all-gather/reduce-scatter EP transport")
     p.add_argument("--disable_fused_optimizer", action="store_true", help="Use NCCL collectives in the optimizer step")
     p.add_argument("--router_z_loss_coef", type=float, default=0.0)
+    p.add_argument("--use_linear_cross_entropy", action="store_true",
+                   help="Loss and its gradients straight from the hidden states and the LM head's weight: the logits are "
+                        "never in memory (without pipeline stages and tensor parallelism; ignored otherwise)")
+    p.add_argument("--opt_use_list_clipping", action="store_true",
+                   help="With --opt_use_pt_optimizer: gradient norm and clipping in one call over all gradients")
     p.add_argument("--moe_capacity_factor", type=float, default=None,
                    help="0 (default): expert-parallel activation buffers sized from each layer's routed counts, nothing "
                         "is ever dropped; > 0: fixed buffers of that multiple of the balanced share (no host read per "
@@ -353,6 +358,7 @@ def main(argv=None):
         weight_decay=args.weight_decay, beta1=args.beta1, beta2=args.beta2, eps=args.eps, warmup_steps=args.warmup_steps,
         opt_grad_acc_steps=args.opt_grad_acc_steps,
         opt_disable_delayed_grad_clipping=args.opt_disable_delayed_grad_clipping,
+        use_linear_cross_entropy=args.use_linear_cross_entropy, opt_use_list_clipping=args.opt_use_list_clipping,
         opt_use_allreduce_for_grad_acc=args.opt_use_allreduce_for_grad_acc,
         opt_use_allreduce_for_param_gather=args.opt_use_allreduce_for_param_gather,
         opt_use_chunked_allreduce=args.opt_use_chunked_allreduce, use_fused_optimizer=not args.disable_fused_optimizer,

@@ -94,6 +94,8 @@ struct GemmParams {
   float* ce_part;
   long long ce_part_ld;
   int* ce_flags;               // [0] any row block flagged, [1 + b] row block b (128 rows) flagged
+  float ce_grow;               // see epilogue_ce
+  int ce_overlap;              // the launch before this one may still be running: wait for it before its results are read
   int ce_repair;               // only the flagged row blocks, with their rows' recorded maxima as references
   int ce_store;                // the exponentials are written to C
 };
@@ -563,6 +565,10 @@ __device__ __forceinline__ bool ce_skip_tile(const GemmParams& p, const TileInfo
 // bits before it, and e keeps bf16's relative precision however small it is.  Columns past N and rows without a target
 // give zeros.  A row whose logits exceed the reference by more than CE_RANGE has its largest logit recorded in ce_max
 // and its row block flagged; a second launch (ce_repair) computes those blocks again against the recorded maxima.
+// The tensor cores truncate as they add: against the exact sum a logit of H terms of random sign comes out smaller by
+// 1.4e-8 of itself for every 16 terms (measured: 4.0e-7 at H = 512, 1.8e-6 at 2048, 6.9e-6 at 7168; up to 6e-8 where all
+// terms have one sign), and a mean loss would keep that bias.  ce_grow = 1 + 1.4e-8 H / 16 gives it back in the
+// multiply-add that takes the difference, which halves the logits' rms error (2.1e-6 to 1.1e-6 at H = 2048).
 // CE_RANGE: sums of 2^31 terms of e^40 = 2.4e17 stay below 1e27, far inside fp32 and bf16, and so does their inverse.
 constexpr float CE_RANGE = 40.f;
 template <int BLOCK_N>
@@ -577,6 +583,7 @@ __device__ __forceinline__ void epilogue_ce(const GemmParams& p, const CUtensorM
   const int tcol = live ? static_cast<int>(target) - ti.n0 : -1;
   const float ref = live ? ce_row_ref(p, row) : 0.f;
   const float2 neg_ref = make_float2(-ref, -ref);
+  const float2 grow = make_float2(p.ce_grow, p.ce_grow);
   const float2 log2e = make_float2(1.4426950408889634f, 1.4426950408889634f);
   float top = -INFINITY;
   float2 sum = make_float2(0.f, 0.f);
@@ -599,7 +606,7 @@ __device__ __forceinline__ void epilogue_ce(const GemmParams& p, const CUtensorM
     for (int i = 0; i < 32; ++i) {
       const float2 l = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
       top = max3(top, l.x, l.y);
-      const float2 d = mul2(add2(l, neg_ref), log2e);
+      const float2 d = mul2(fma2(l, grow, neg_ref), log2e);
       r[2 * i] = __float_as_uint(ex2_approx(d.x));
       r[2 * i + 1] = __float_as_uint(ex2_approx(d.y));
     }
@@ -976,6 +983,9 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
     }
   } else if (warp < 6) {
     // ------------------------------------------------------------ epilogue (warps 2..5)
+    if constexpr (EPI == EPI_CE) {
+      if (p.ce_overlap) grid_dependency_wait();
+    }
     const int lane_group = warp & 3;  // TMEM lanes [32*lane_group, +32) belong to this warp
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -1291,6 +1301,9 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
     }
   } else if (warp < 6) {
     // ------------------------------------------------------------ epilogue (warps 2..5 of both CTAs, own 128 rows)
+    if constexpr (EPI == EPI_CE) {
+      if (p.ce_overlap) grid_dependency_wait();
+    }
     const int lane_group = warp & 3;
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -1458,6 +1471,24 @@ struct TensorMaps {
   CUtensorMap a, b, b2, c, c2;
 };
 
+// A launch that may start once the one before it on the stream has let it (griddepcontrol.launch_dependents).
+template <bool PEER>
+static int launch_overlapped(void (*kernel)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, PeerArg<PEER>, GemmParams),
+                             int grid, int threads, int smem, cudaStream_t stream, const TensorMaps& tm,
+                             const PeerArg<PEER>& peers, const GemmParams& p) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, tm.a, tm.b, tm.b2, tm.c, tm.c2, peers, p) == cudaSuccess ? 0 : -4;
+}
+
 template <int BLOCK_N, bool PEER, int EPI>
 static int launch(const TensorMaps& tm, const PeerArg<PEER>& peers, const GemmParams& p, int num_sms, cudaStream_t stream) {
   using L = SmemLayout<BLOCK_N>;
@@ -1476,6 +1507,10 @@ static int launch(const TensorMaps& tm, const PeerArg<PEER>& peers, const GemmPa
   const long long tiles = nm * nn * (p.mode == OLB_GEMM_RAGGED_K ? p.num_experts : (p.k_splits > 1 ? p.k_splits : 1));
   int grid = static_cast<int>(tiles < num_sms ? tiles : num_sms);
   if (grid <= 0) return 0;
+  if constexpr (EPI == EPI_CE) {
+    if (p.ce_overlap)
+      return launch_overlapped(gemm_bf16_kernel<BLOCK_N, PEER, EPI>, grid, NUM_THREADS, L::TOTAL, stream, tm, peers, p);
+  }
   gemm_bf16_kernel<BLOCK_N, PEER, EPI><<<grid, PEER ? NUM_THREADS_STAGED : NUM_THREADS, L::TOTAL, stream>>>(
       tm.a, tm.b, tm.b2, tm.c, tm.c2, peers, p);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
@@ -1501,6 +1536,10 @@ static int launch_pair(const TensorMaps& tm, const PeerArg<PEER>& peers, const G
   const int max_pairs = num_sms / 2;
   const int pairs = static_cast<int>(tiles < max_pairs ? tiles : max_pairs);
   if (pairs <= 0) return 0;
+  if constexpr (EPI == EPI_CE) {
+    if (p.ce_overlap)
+      return launch_overlapped(gemm_bf16_pair_kernel<PEER, EPI>, 2 * pairs, NUM_THREADS, L::TOTAL, stream, tm, peers, p);
+  }
   gemm_bf16_pair_kernel<PEER, EPI><<<2 * pairs, PEER ? NUM_THREADS_STAGED : NUM_THREADS, L::TOTAL, stream>>>(
       tm.a, tm.b, tm.b2, tm.c, tm.c2, peers, p);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
@@ -1558,12 +1597,31 @@ static int device_sm_count() {
 
 }  // namespace olb
 
-// Columns per statistics tile of the cross-entropy product: 256 (CTA pairs, or one CTA for fewer than 256 rows) while
-// that gives every SM work, else narrower tiles, so that a small batch still spreads the weight over the SMs.
-extern "C" int olb_gemm_ce_block_n(int M, int N) {
-  (void)M;
-  (void)N;
-  return 256;
+// Tiles of the cross-entropy product: CTA pairs on 256 x 256, or one CTA on 128 x {256, 128, 64}, whichever takes the
+// fewest column-steps counted in whole waves over the SMs, with 32 columns for a tile's own start and end and 15 % for
+// what a single CTA loses against a pair.  So a short batch spreads the weight's rows over all SMs (one row against
+// 128256 x 4096: 195 us with 256 columns, four waves of 148 for 501 tiles) and a long one takes pairs.
+extern "C" int olb_gemm_ce_block_n(int M, int N, int* pair) {
+  using namespace olb;
+  const long long sms = device_sm_count() > 1 ? device_sm_count() : 148;
+  auto waves = [](long long tiles, long long workers) { return static_cast<double>((tiles + workers - 1) / workers); };
+  const long long m = (M + 127) / 128;
+  int best = 256, with_pair = 0;
+  double least = 1e300;
+  if (M >= 256 && pair_kernel_enabled()) {
+    least = waves((M + 255) / 256 * ((N + 255ll) / 256), sms / 2) * (256 + 32);
+    with_pair = 1;
+  }
+  for (int bn : {256, 128, 64}) {
+    const double cost = waves(m * ((N + bn - 1ll) / bn), sms) * (1.15 * bn + 32);
+    if (cost < least) {
+      least = cost;
+      best = bn;
+      with_pair = 0;
+    }
+  }
+  if (pair) *pair = with_pair;
+  return best;
 }
 
 extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
@@ -1573,7 +1631,7 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
       (reinterpret_cast<uintptr_t>(d->B) & 15) || (reinterpret_cast<uintptr_t>(d->C) & 15))
     return -10;
   const int epi = d->epilogue;
-  int block_n = d->block_n;
+  int block_n = d->block_n, ce_pair = 0;
   if (epi == OLB_EPI_SWIGLU) {
     // N = width of act; B / B2 = gate / up weights (K-major, same layout); C = gate | up [rows, 2 N]; C2 = act [rows, N]
     if (d->N % 128 || d->B2 == nullptr || d->C2 == nullptr || d->b_mn_major || d->a_mn_major || d->accumulate ||
@@ -1595,9 +1653,9 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
     if (d->a_mn_major || d->b_mn_major || d->accumulate || d->out_fp32 || d->mode != OLB_GEMM_DENSE || d->n_peers ||
         d->k_split || d->k_splits > 1 || d->ce_targets == nullptr || d->ce_ref == nullptr ||
         (d->ce_repair && (d->ce_flags == nullptr || d->ce_max == nullptr)) || (d->ce_flags != nullptr && d->ce_max == nullptr) ||
-        (d->ce_part != nullptr && d->ce_part_ld < d->M))
+        (d->ce_part != nullptr && d->ce_part_ld < d->M) || (d->ce_overlap && d->ce_repair))
       return -18;
-    block_n = olb_gemm_ce_block_n(d->M, d->N);
+    block_n = olb_gemm_ce_block_n(d->M, d->N, &ce_pair);
   } else if (epi == OLB_EPI_ROWSCALE) {
     if (d->row_scale == nullptr || d->accumulate || d->out_fp32 || d->mode != OLB_GEMM_DENSE || d->n_peers || d->k_splits > 1 ||
         block_n != 0)
@@ -1619,8 +1677,9 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   // (ragged-M: only when the caller padded the expert groups to 256 rows; the dense all-gather / reduce-scatter
   // variants, whose peers own multiples of 128 rows, stay on the single-CTA kernel)
   const bool pair_shape = d->block_n == 0 && block_n == 256 && d->blk_range == nullptr && d->M >= 256 && num_sms >= 2 &&
-                          (epi == OLB_EPI_SWIGLU || epi == OLB_EPI_SWIGLU_BWD || epi == OLB_EPI_CE || d->N % 256 == 0 ||
-                           d->N >= 2048);
+                          (epi == OLB_EPI_SWIGLU || epi == OLB_EPI_SWIGLU_BWD || (epi == OLB_EPI_CE && ce_pair) ||
+                           (epi != OLB_EPI_CE && (d->N % 256 == 0 || d->N >= 2048 ||
+                                                  (d->wide_tiles && (256 - d->N % 256) * 8 <= d->N))));
   const bool use_pair = pair_kernel_enabled() && pair_shape &&
                         (d->mode == OLB_GEMM_RAGGED_M ? (d->pair_rows != 0 && d->M % 256 == 0)
                                                       : ((d->n_peers == 0 || d->B_peers != nullptr) &&
@@ -1707,6 +1766,8 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   p.ce_part_ld = d->ce_part_ld;
   p.ce_flags = d->ce_flags;
   p.ce_repair = d->ce_repair;
+  p.ce_overlap = d->ce_overlap;
+  p.ce_grow = static_cast<float>(1.0 + 1.4e-8 / 16 * d->K);
   p.ce_store = epi == OLB_EPI_CE && d->C != nullptr;
   p.c_part_rows = d->mode == OLB_GEMM_RAGGED_K ? d->M : 0;
   p.k_splits = 1;

@@ -3,8 +3,10 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <torch/csrc/autograd/python_variable.h>
+
 #include <algorithm>
-#include <tuple>
+#include <functional>
 
 #include "olb_api.h"
 
@@ -26,9 +28,15 @@ bool no_self_overlap(const at::Tensor& t) {
 
 // The norm as a 0-dim fp32 tensor; nothing when a tensor's type is not one the kernels read (the caller has another way).
 // Dense tensors are read, and scaled, where they lie, whatever the order of their axes; the others through a copy.
-c10::optional<at::Tensor> grad_clip(const std::vector<at::Tensor>& grads, bool inf_norm, bool scale, double max_norm, double eps) {
-  TORCH_CHECK_VALUE(!grads.empty(), "no gradients");
-  const at::Device device = grads[0].device();
+c10::optional<at::Tensor> grad_clip(const pybind11::list& items, bool inf_norm, bool scale, double max_norm, double eps) {
+  TORCH_CHECK_VALUE(!items.empty(), "no gradients");
+  std::vector<std::reference_wrapper<const at::Tensor>> grads;  // the list holds them for the length of the call
+  grads.reserve(items.size());
+  for (const pybind11::handle& item : items) {
+    TORCH_CHECK_TYPE(THPVariable_Check(item.ptr()), "gradients must be tensors");
+    grads.emplace_back(THPVariable_Unpack(item.ptr()));
+  }
+  const at::Device device = grads[0].get().device();
   std::vector<olb_clip_tensor> list;
   list.reserve(grads.size());
   std::vector<std::pair<at::Tensor, at::Tensor>> copies;   // a tensor that is not dense, and its copy

@@ -27,16 +27,48 @@ namespace olb {
 constexpr int LCE_THREADS = 256;
 constexpr int LCE_WARPS = LCE_THREADS / 32;
 
-// ref[r] = x_r . w_t, one warp per row.
+// How many of the whole batch's n targets lie in [0, V): integers, so their order does not matter.
+__device__ __forceinline__ void lce_count(const long long* __restrict__ targets, long long n, int V, float* __restrict__ count,
+                                          float* __restrict__ inv_count) {
+  __shared__ int s[LCE_WARPS];
+  int c = 0;  // n < 2^31
+#pragma unroll 4
+  for (long long i = threadIdx.x; i < n; i += LCE_THREADS) {
+    const long long t = targets[i];
+    c += (t >= 0 && t < V) ? 1 : 0;
+  }
+  c = __reduce_add_sync(0xffffffffu, c);
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = c;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int total = 0;
+    for (int i = 0; i < LCE_WARPS; ++i) total += s[i];
+    *count = static_cast<float>(total);
+    *inv_count = total > 0 ? 1.f / static_cast<float>(total) : 0.f;
+  }
+}
+
+// ref[r] = x_r . w_t: one warp per row, or the block's eight for one row when there are few (a single row of 4096:
+// 6.7 us with one warp).  The last block counts the targets (`count` set).
+template <bool FEW>
 __global__ void __launch_bounds__(LCE_THREADS)
 lce_prep_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, const __nv_bfloat16* __restrict__ w, long long ldw,
                 const long long* __restrict__ targets, int rows, int H, int V, float* __restrict__ ref,
-                unsigned* __restrict__ ce_max, int* __restrict__ ce_flags, unsigned* __restrict__ ticket) {
-  const int lane = threadIdx.x & 31;
-  const int row = blockIdx.x * LCE_WARPS + (threadIdx.x >> 5);
+                unsigned* __restrict__ ce_max, int* __restrict__ ce_flags, unsigned* __restrict__ ticket,
+                const long long* __restrict__ all_targets, long long n_all, float* __restrict__ count) {
+  // the product may start: nothing of it but its epilogue needs what this kernel writes
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (count != nullptr && blockIdx.x == gridDim.x - 1) {
+    lce_count(all_targets, n_all, V, count, count + 1);
+    return;
+  }
+  __shared__ float s_part[LCE_WARPS];
+  const int warp = threadIdx.x >> 5, lane = FEW ? threadIdx.x : threadIdx.x & 31;
+  constexpr int LANES = FEW ? LCE_THREADS : 32;
+  const int row = FEW ? blockIdx.x : blockIdx.x * LCE_WARPS + warp;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     ce_flags[0] = 0;
-    if (ticket) *ticket = 0;
+    *ticket = 0;
   }
   if (row >= rows) return;
   const long long t = targets[row];
@@ -47,7 +79,7 @@ lce_prep_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, const __nv_b
     const int vecs = H / 8;
     float2 s0 = make_float2(0.f, 0.f), s1 = s0;
 #pragma unroll 4
-    for (int i = lane; i < vecs; i += 32) {
+    for (int i = lane; i < vecs; i += LANES) {
       const uint4 u = a[i], v = b[i];
       s0 = fma2(unpack_bf16(u.x), unpack_bf16(v.x), s0);
       s1 = fma2(unpack_bf16(u.y), unpack_bf16(v.y), s1);
@@ -56,6 +88,13 @@ lce_prep_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, const __nv_b
     }
     acc = warp_sum((s0.x + s0.y) + (s1.x + s1.y));
   }
+  if (FEW) {
+    if ((threadIdx.x & 31) == 0) s_part[warp] = acc;
+    __syncthreads();
+    acc = 0.f;
+#pragma unroll
+    for (int i = 0; i < LCE_WARPS; ++i) acc += s_part[i];
+  }
   if (lane == 0) {
     ref[row] = acc;
     ce_max[row] = 0;
@@ -63,26 +102,21 @@ lce_prep_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, const __nv_b
   }
 }
 
-// One block: the counts are integers, so their order does not matter.
-__global__ void __launch_bounds__(1024)
-lce_count_kernel(const long long* __restrict__ targets, long long n, int V, float* __restrict__ count,
-                 float* __restrict__ inv_count) {
-  __shared__ int s[32];
-  long long c = 0;
-  for (long long i = threadIdx.x; i < n; i += 1024) {
-    const long long t = targets[i];
-    c += (t >= 0 && t < V) ? 1 : 0;
+// xs[row, :] = bf16(f * x[row, :]), by one warp.  A row without a target (f = 0) gives zeros whatever it holds.
+__device__ __forceinline__ void lce_scale_row(const void* x, long long ldx, void* xs, long long row, int H, float f, int lane) {
+  const int vecs = H / 8;
+  uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(xs) + row * H);
+  if (f == 0.f) {
+    for (int i = lane; i < vecs; i += 32) dst[i] = make_uint4(0, 0, 0, 0);
+    return;
   }
-  int ci = static_cast<int>(c);  // n < 2^31
-  ci = __reduce_add_sync(0xffffffffu, ci);
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = ci;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    const int total = __reduce_add_sync(0xffffffffu, s[threadIdx.x]);
-    if (threadIdx.x == 0) {
-      *count = static_cast<float>(total);
-      *inv_count = total > 0 ? 1.f / static_cast<float>(total) : 0.f;
-    }
+  const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(x) + row * ldx);
+#pragma unroll 4
+  for (int i = lane; i < vecs; i += 32) {
+    const uint4 u = src[i];
+    const float2 a = unpack_bf16(u.x), b = unpack_bf16(u.y), c = unpack_bf16(u.z), e = unpack_bf16(u.w);
+    dst[i] = make_uint4(pack_bf16(f * a.x, f * a.y), pack_bf16(f * b.x, f * b.y), pack_bf16(f * c.x, f * c.y),
+                        pack_bf16(f * e.x, f * e.y));
   }
 }
 
@@ -94,37 +128,38 @@ __device__ __forceinline__ float lce_patch_row(__nv_bfloat16* entry, float S, fl
   return rounded > 0.f && rounded <= FLT_MAX ? inv_z * (S / rounded) : inv_z;
 }
 
-// Block: 32 rows.  Its warps share the tiles' sums (lane = row, so that a load is 128 consecutive bytes), the first
-// warp finishes the rows, then the warps scale the rows of X.
+// Block: 8 rows (a 32-byte sector of every tile's sums) x 32 tiles at a time; eight threads finish the rows, then each
+// warp scales one row of X.  (32 rows per block left half of the SMs without one: 29 us for 8192 x 2048, V = 50304.)
+constexpr int LCE_ROWS = 8;
 __global__ void __launch_bounds__(LCE_THREADS)
 lce_finish_kernel(const olb_lce_finish_desc d) {
-  __shared__ float s_sum[LCE_WARPS][32];
-  __shared__ float s_factor[32];
+  constexpr int TILES = LCE_THREADS / LCE_ROWS;
+  __shared__ float s_sum[TILES][LCE_ROWS];
+  __shared__ float s_factor[LCE_ROWS];
   __shared__ bool s_last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row0 = blockIdx.x * 32;
-  const int row = row0 + lane;
+  const int row0 = blockIdx.x * LCE_ROWS;
+  const int sub = threadIdx.x % LCE_ROWS, row = row0 + sub;
   const bool ok = row < d.rows;
+  const long long t = ok ? d.targets[row] : -1;
   {
     float s = 0.f;
-    const long long t = ok ? d.targets[row] : -1;
     if (t >= 0 && t < d.V) {
       const float* p = d.part + row;
 #pragma unroll 8
-      for (int i = warp; i < d.ntiles; i += LCE_WARPS) s += p[i * d.part_ld];
+      for (int i = threadIdx.x / LCE_ROWS; i < d.ntiles; i += TILES) s += p[i * d.part_ld];
     }
-    s_sum[warp][lane] = s;
+    s_sum[threadIdx.x / LCE_ROWS][sub] = s;
   }
   __syncthreads();
-  if (warp == 0) {
+  if (threadIdx.x < LCE_ROWS) {
     float factor = 0.f;
     if (ok) {
-      const long long t = d.targets[row];
       float loss = 0.f, prob = 0.f, lse = 0.f;
       if (t >= 0 && t < d.V) {
         float S = 0.f;
 #pragma unroll
-        for (int i = 0; i < LCE_WARPS; ++i) S += s_sum[i][lane];
+        for (int i = 0; i < TILES; ++i) S += s_sum[i][sub];
         const float lt = d.ref[row];
         const unsigned m = d.ce_max[row];
         float z;
@@ -147,27 +182,12 @@ lce_finish_kernel(const olb_lce_finish_desc d) {
       if (d.lse) d.lse[row] = lse;
       if (d.factor) d.factor[row] = factor;
     }
-    s_factor[lane] = factor;
+    s_factor[sub] = factor;
   }
   __syncthreads();
   if (d.xs) {
-    const int vecs = d.H / 8;
-    for (int r = warp; r < 32 && row0 + r < d.rows; r += LCE_WARPS) {
-      const float f = s_factor[r];
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(d.x) + (row0 + r) * d.ldx);
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(d.xs) + static_cast<long long>(row0 + r) * d.H);
-      if (f == 0.f) {  // a row without a target gives zeros whatever it holds
-        for (int i = lane; i < vecs; i += 32) dst[i] = make_uint4(0, 0, 0, 0);
-        continue;
-      }
-#pragma unroll 4
-      for (int i = lane; i < vecs; i += 32) {
-        const uint4 u = src[i];
-        const float2 a = unpack_bf16(u.x), b = unpack_bf16(u.y), c = unpack_bf16(u.z), e = unpack_bf16(u.w);
-        dst[i] = make_uint4(pack_bf16(f * a.x, f * a.y), pack_bf16(f * b.x, f * b.y), pack_bf16(f * c.x, f * c.y),
-                            pack_bf16(f * e.x, f * e.y));
-      }
-    }
+    static_assert(LCE_WARPS == LCE_ROWS, "one warp per row");
+    if (row0 + warp < d.rows) lce_scale_row(d.x, d.ldx, d.xs, row0 + warp, d.H, s_factor[warp], lane);
   }
   if (d.total == nullptr) return;
   // the last block to arrive sums the rows' losses, in a fixed order
@@ -180,11 +200,11 @@ lce_finish_kernel(const olb_lce_finish_desc d) {
   float acc = 0.f;
   for (long long i = threadIdx.x; i < d.n_all; i += LCE_THREADS) acc += __ldcg(d.loss_all + i);
   acc = warp_sum(acc);
-  if (lane == 0) s_sum[0][warp] = acc;
+  if (lane == 0) s_factor[warp] = acc;
   __syncthreads();
   if (threadIdx.x == 0) {
     float sum = 0.f;
-    for (int i = 0; i < LCE_WARPS; ++i) sum += s_sum[0][i];
+    for (int i = 0; i < LCE_WARPS; ++i) sum += s_factor[i];
     // a division, as a mean is defined: 0 / 0 where no row has a target
     *d.total = d.total_scale ? sum / *d.total_scale : sum;
   }
@@ -212,21 +232,7 @@ lce_scale_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, const 
   const float f0 = factor[row];
   const float f = f0 == 0.f ? 0.f : f0 * grad[row * grad_stride];
   if (lane == 0) row_factor[row] = f;
-  if (!xs) return;
-  const int vecs = H / 8;
-  uint4* dst = reinterpret_cast<uint4*>(xs + static_cast<long long>(row) * H);
-  if (f == 0.f) {
-    for (int i = lane; i < vecs; i += 32) dst[i] = make_uint4(0, 0, 0, 0);
-    return;
-  }
-  const uint4* src = reinterpret_cast<const uint4*>(x + row * ldx);
-#pragma unroll 4
-  for (int i = lane; i < vecs; i += 32) {
-    const uint4 u = src[i];
-    const float2 a = unpack_bf16(u.x), b = unpack_bf16(u.y), c = unpack_bf16(u.z), e = unpack_bf16(u.w);
-    dst[i] = make_uint4(pack_bf16(f * a.x, f * a.y), pack_bf16(f * b.x, f * b.y), pack_bf16(f * c.x, f * c.y),
-                        pack_bf16(f * e.x, f * e.y));
-  }
+  if (xs) lce_scale_row(x, ldx, xs, row, H, f, lane);
 }
 
 // 8 columns per thread; the parts are summed in their order.
@@ -288,26 +294,25 @@ using namespace olb;
 
 extern "C" int olb_lce_prep(const void* x, long long ldx, const void* w, long long ldw, const long long* targets, int rows,
                             int H, int V, float* ref, unsigned* ce_max, int* ce_flags, unsigned* ticket,
-                            cudaStream_t stream) {
-  if (H % 8 || ldx % 8 || ldw % 8 || misaligned(x) || misaligned(w)) return -1;
+                            const long long* all_targets, long long n_all, float* count, cudaStream_t stream) {
+  if (H % 8 || ldx % 8 || ldw % 8 || misaligned(x) || misaligned(w) || n_all >= (1ll << 31)) return -1;
   if (rows <= 0) return 0;
-  lce_prep_kernel<<<(rows + LCE_WARPS - 1) / LCE_WARPS, LCE_THREADS, 0, stream>>>(
-      static_cast<const __nv_bfloat16*>(x), ldx, static_cast<const __nv_bfloat16*>(w), ldw, targets, rows, H, V, ref, ce_max,
-      ce_flags, ticket);
-  return launched();
-}
-
-extern "C" int olb_lce_count(const long long* targets, long long n, int V, float* count, float* inv_count,
-                             cudaStream_t stream) {
-  if (n >= (1ll << 31)) return -1;
-  lce_count_kernel<<<1, 1024, 0, stream>>>(targets, n, V, count, inv_count);
+  const auto* xb = static_cast<const __nv_bfloat16*>(x);
+  const auto* wb = static_cast<const __nv_bfloat16*>(w);
+  const int extra = count != nullptr ? 1 : 0;
+  if (rows <= 148)
+    lce_prep_kernel<true><<<rows + extra, LCE_THREADS, 0, stream>>>(xb, ldx, wb, ldw, targets, rows, H, V, ref, ce_max,
+                                                                    ce_flags, ticket, all_targets, n_all, count);
+  else
+    lce_prep_kernel<false><<<(rows + LCE_WARPS - 1) / LCE_WARPS + extra, LCE_THREADS, 0, stream>>>(
+        xb, ldx, wb, ldw, targets, rows, H, V, ref, ce_max, ce_flags, ticket, all_targets, n_all, count);
   return launched();
 }
 
 extern "C" int olb_lce_finish(const olb_lce_finish_desc* d, cudaStream_t stream) {
   if ((d->xs && (d->H % 8 || d->ldx % 8 || misaligned(d->x) || misaligned(d->xs))) || (d->total && !d->ticket)) return -1;
   if (d->rows <= 0) return 0;
-  lce_finish_kernel<<<(d->rows + 31) / 32, LCE_THREADS, 0, stream>>>(*d);
+  lce_finish_kernel<<<(d->rows + LCE_ROWS - 1) / LCE_ROWS, LCE_THREADS, 0, stream>>>(*d);
   return launched();
 }
 

@@ -24,6 +24,14 @@ inline void check(int rc, const char* what) { TORCH_CHECK(rc == 0, std::string(w
 
 enum { MEAN = 0, SUM = 1, NONE = 2 };
 
+// What forward leaves to backward: with one piece the exponentials and row factors, with several the gradients of a
+// scalar loss (dx and dw in fp32; undefined where not wanted) or the rows' 1 - p_target and log-sum-exp.
+enum { PIECE = 0, SCALE = 1, AGAIN = 2 };
+struct Kept {
+  int64_t kind = PIECE;
+  at::Tensor a, b;
+};
+
 int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
 struct Problem {
@@ -58,7 +66,7 @@ void* row_ptr(const at::Tensor& t, int64_t row) { return static_cast<char*>(t.da
 // fp32 partial products written and read once at 4.5 TB/s plus the launch that sums them.
 int split_parts(int64_t M, int64_t N, int64_t K) {
   int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  const bool pair = M >= 256 && (N % 256 == 0 || N >= 2048);
+  const bool pair = M >= 256 && (N % 256 == 0 || N >= 2048 || (256 - N % 256) * 8 <= N);
   const int64_t tm = pair ? 256 : 128, tn = N > 128 ? 256 : (N > 64 ? 128 : 64), workers = pair ? sms / 2 : sms;
   const int64_t tiles = ((M + tm - 1) / tm) * ((N + tn - 1) / tn), kb = (K + 63) / 64;
   const double block_us = 2.0 * tm * tn * 64 * workers / 1.5e9;
@@ -78,7 +86,7 @@ int split_parts(int64_t M, int64_t N, int64_t K) {
 
 // e = exp(l - ref) of one piece (and the sums of its tiles), then the row blocks that need another reference.
 void product(const Problem& p, int64_t r0, int64_t rows, const float* ref, unsigned* top, int* flags, float* part,
-             int64_t part_ld, void* E) {
+             int64_t part_ld, void* E, bool behind_prep) {
   olb_gemm_desc d{};
   d.A = row_ptr(p.x, r0);
   d.B = p.w.data_ptr();
@@ -99,8 +107,10 @@ void product(const Problem& p, int64_t r0, int64_t rows, const float* ref, unsig
   d.ce_flags = flags;
   d.ce_part = part;
   d.ce_part_ld = part_ld;
+  d.ce_overlap = behind_prep;
   check(olb_gemm_bf16(&d, p.stream), "olb_gemm_bf16 (cross entropy)");
   if (flags) {
+    d.ce_overlap = 0;
     d.ce_repair = 1;
     check(olb_gemm_bf16(&d, p.stream), "olb_gemm_bf16 (cross entropy, repair)");
   }
@@ -120,6 +130,7 @@ void input_gradient(const Problem& p, int64_t r0, int64_t rows, const void* E, c
   d.N = static_cast<int>(p.H);
   d.K = static_cast<int>(p.V);
   d.b_mn_major = 1;
+  d.wide_tiles = 1;
   d.status = p.status;
   d.ldc = p.H;
   if (parts == 1) {
@@ -156,6 +167,7 @@ void weight_gradient(const Problem& p, int64_t rows, const void* E, const void* 
   d.N = static_cast<int>(p.H);
   d.K = static_cast<int>(rows);
   d.a_mn_major = d.b_mn_major = 1;
+  d.wide_tiles = 1;
   d.status = p.status;
   d.out_fp32 = dw.scalar_type() == at::kFloat;
   if (d.out_fp32)
@@ -175,10 +187,9 @@ at::Tensor weight_gradient_out(const Problem& p, const c10::optional<at::Tensor>
   return *dw_out;
 }
 
-// Returns the loss (a scalar, or [T] for NONE) and what the backward needs: with one piece {E, factor}; with several
-// {dx, dw32} for a scalar loss (undefined where not wanted), {prob, lse} for losses per row.
-std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, int64_t reduction,
-                                      bool need_dx, bool need_dw, int64_t max_bytes, const at::Tensor& status) {
+// The loss: a scalar, or [T] for NONE.
+at::Tensor linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, int64_t reduction,
+                         bool need_dx, bool need_dw, int64_t max_bytes, const at::Tensor& status, Kept& kept) {
   TORCH_CHECK(reduction >= MEAN && reduction <= NONE);
   c10::cuda::CUDAGuard guard(x.device());
   const Problem p = make_problem(x, w, targets, status);
@@ -187,15 +198,14 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, 
   if (p.T == 0) {
     at::Tensor out = reduction == NONE ? at::empty({0}, f32)
                                        : at::full({}, reduction == MEAN ? std::numeric_limits<double>::quiet_NaN() : 0.0, f32);
-    return {out, at::empty({0, p.lde}, x.options()), at::empty({0}, f32)};
+    kept = {PIECE, at::empty({0, p.lde}, x.options()), at::empty({0}, f32)};
+    return out;
   }
-  const int64_t tile = olb_gemm_ce_block_n(static_cast<int>(p.T), static_cast<int>(p.V));
   int64_t rows_max = piece_rows(p.T, grad ? 2 * p.lde : 4 * ((p.V + 63) / 64), max_bytes);
   const bool single = rows_max >= p.T;
   const bool store = grad && (single || reduction != NONE);   // several pieces of losses per row: exponentials again later
   if (grad && !single && reduction == NONE) rows_max = piece_rows(p.T, 4 * ((p.V + 63) / 64), max_bytes);
   const int64_t ntiles_most = (p.V + 63) / 64;
-  (void)tile;
 
   at::Tensor loss_rows = at::empty({p.T}, f32);
   at::Tensor out = reduction == NONE ? loss_rows : at::empty({}, f32);
@@ -224,15 +234,14 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, 
     prob = at::empty({p.T}, f32);
     lse = at::empty({p.T}, f32);
   }
-  if (reduction == MEAN)
-    check(olb_lce_count(ptr_i64(p.targets, 0), p.T, static_cast<int>(p.V), count, count + 1, p.stream), "olb_lce_count");
   for (int64_t r0 = 0; r0 < p.T; r0 += rows_max) {
     const int64_t rows = std::min(rows_max, p.T - r0);
-    const int bn = olb_gemm_ce_block_n(static_cast<int>(rows), static_cast<int>(p.V));
+    const int bn = olb_gemm_ce_block_n(static_cast<int>(rows), static_cast<int>(p.V), nullptr);
     check(olb_lce_prep(row_ptr(x, r0), x.stride(0), w.data_ptr(), w.stride(0), ptr_i64(p.targets, r0), static_cast<int>(rows),
-                       static_cast<int>(p.H), static_cast<int>(p.V), ref, top, flags, ticket, p.stream),
+                       static_cast<int>(p.H), static_cast<int>(p.V), ref, top, flags, ticket, ptr_i64(p.targets, 0), p.T,
+                       reduction == MEAN && r0 == 0 ? count : nullptr, p.stream),
           "olb_lce_prep");
-    product(p, r0, rows, ref, top, flags, part.data_ptr<float>(), rows_max, store ? E.data_ptr() : nullptr);
+    product(p, r0, rows, ref, top, flags, part.data_ptr<float>(), rows_max, store ? E.data_ptr() : nullptr, true);
     olb_lce_finish_desc f{};
     f.part = part.data_ptr<float>();
     f.part_ld = rows_max;
@@ -272,10 +281,10 @@ std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, 
       if (need_dw) weight_gradient(p, rows, E.data_ptr(), xs.data_ptr(), dw32, r0 > 0);
     }
   }
-  if (!grad) return {out};
-  if (in_forward) return {out, dx, dw32};
-  if (store) return {out, E, factor};
-  return {out, prob, lse};
+  if (in_forward) kept = {SCALE, dx, dw32};
+  else if (store) kept = {PIECE, E, factor};
+  else kept = {AGAIN, prob, lse};
+  return out;
 }
 
 // One piece: E and factor as the forward left them; grad is a scalar or [T].  Returns {dx, dw} (undefined where not
@@ -307,21 +316,21 @@ std::vector<at::Tensor> linear_ce_bwd(const at::Tensor& x, const at::Tensor& w, 
 }
 
 // Several pieces of a scalar loss: the gradients of the forward times the incoming gradient.
-std::vector<at::Tensor> linear_ce_bwd_scale(const c10::optional<at::Tensor>& dx_in, const c10::optional<at::Tensor>& dw32,
-                                            const at::Tensor& grad, const c10::optional<at::Tensor>& dw_out, bool accumulate) {
-  const at::Tensor& any = dx_in.has_value() ? *dx_in : *dw32;
+std::vector<at::Tensor> linear_ce_bwd_scale(const at::Tensor& dx_in, const at::Tensor& dw32, const at::Tensor& grad,
+                                            const c10::optional<at::Tensor>& dw_out, bool accumulate) {
+  const at::Tensor& any = dx_in.defined() ? dx_in : dw32;
   c10::cuda::CUDAGuard guard(any.device());
   TORCH_CHECK(grad.scalar_type() == at::kFloat && grad.numel() == 1 && grad.device() == any.device());
   at::Tensor dx, dw;
-  if (dx_in.has_value()) {
-    dx = at::empty_like(*dx_in);
-    check(olb_lce_scale_out(dx_in->data_ptr(), 1, dx.numel(), grad.data_ptr<float>(), dx.data_ptr(), 0, cur_stream()), "olb_lce_scale_out");
+  if (dx_in.defined()) {
+    dx = at::empty_like(dx_in);
+    check(olb_lce_scale_out(dx_in.data_ptr(), 1, dx.numel(), grad.data_ptr<float>(), dx.data_ptr(), 0, cur_stream()), "olb_lce_scale_out");
   }
-  if (dw32.has_value()) {
+  if (dw32.defined()) {
     TORCH_CHECK(!accumulate || dw_out.has_value());
-    dw = dw_out.has_value() ? *dw_out : at::empty(dw32->sizes(), dw32->options().dtype(at::kBFloat16));
-    TORCH_CHECK(dw.scalar_type() == at::kBFloat16 && dw.is_contiguous() && dw.sizes() == dw32->sizes() && dw.device() == dw32->device());
-    check(olb_lce_scale_out(dw32->data_ptr(), 0, dw.numel(), grad.data_ptr<float>(), dw.data_ptr(), accumulate, cur_stream()), "olb_lce_scale_out");
+    dw = dw_out.has_value() ? *dw_out : at::empty(dw32.sizes(), dw32.options().dtype(at::kBFloat16));
+    TORCH_CHECK(dw.scalar_type() == at::kBFloat16 && dw.is_contiguous() && dw.sizes() == dw32.sizes() && dw.device() == dw32.device());
+    check(olb_lce_scale_out(dw32.data_ptr(), 0, dw.numel(), grad.data_ptr<float>(), dw.data_ptr(), accumulate, cur_stream()), "olb_lce_scale_out");
   }
   return {dx, dw};
 }
@@ -348,7 +357,7 @@ std::vector<at::Tensor> linear_ce_bwd_again(const at::Tensor& x, const at::Tenso
   }
   for (int64_t r0 = 0; r0 < p.T; r0 += rows_max) {
     const int64_t rows = std::min(rows_max, p.T - r0);
-    product(p, r0, rows, lse.data_ptr<float>() + r0, nullptr, nullptr, nullptr, 0, E.data_ptr());
+    product(p, r0, rows, lse.data_ptr<float>() + r0, nullptr, nullptr, nullptr, 0, E.data_ptr(), false);
     check(olb_lce_patch(prob.data_ptr<float>() + r0, ptr_i64(p.targets, r0), static_cast<int>(rows), static_cast<int>(p.V),
                         E.data_ptr(), p.lde, factor.data_ptr<float>(), p.stream),
           "olb_lce_patch");
@@ -364,11 +373,95 @@ std::vector<at::Tensor> linear_ce_bwd_again(const at::Tensor& x, const at::Tenso
   return {dx, dw};
 }
 
+// A gradient buffer of ops/functional.py (DirectGrad): `buf`, and `ready` = it holds a gradient of this step already.
+struct GradHolder : torch::CustomClassHolder {
+  pybind11::object obj;
+  explicit GradHolder(pybind11::object o) : obj(std::move(o)) {}
+  ~GradHolder() override {
+    pybind11::gil_scoped_acquire gil;
+    obj = pybind11::object();
+  }
+};
+
+// The autograd node lives here rather than in Python: a training step of a small batch is bound by the host, and the
+// Python form of the same node took 190 us for 65 us of kernels.
+struct LinearCE : torch::autograd::Function<LinearCE> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
+                            const at::Tensor& targets, int64_t reduction, bool need_dx, bool need_dw, int64_t max_bytes,
+                            const at::Tensor& status, const c10::intrusive_ptr<GradHolder>& holder) {
+    Kept kept;
+    at::Tensor out = linear_ce_fwd(x, w, targets, reduction, need_dx, need_dw, max_bytes, status, kept);
+    ctx->save_for_backward({x, w, targets, status, kept.a, kept.b});
+    ctx->saved_data["kind"] = kept.kind;
+    ctx->saved_data["need"] = static_cast<int64_t>(need_dx) + 2 * static_cast<int64_t>(need_dw);
+    ctx->saved_data["max_bytes"] = max_bytes;
+    if (holder) ctx->saved_data["holder"] = c10::IValue::make_capsule(holder);
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "linear_cross_entropy cannot be differentiated twice");
+    const auto saved = ctx->get_saved_variables();
+    const int64_t kind = ctx->saved_data["kind"].toInt(), need = ctx->saved_data["need"].toInt();
+    const bool need_dx = need & 1, need_dw = need & 2;
+    const at::Tensor grad = grads[0].to(at::kFloat).contiguous();
+    c10::optional<at::Tensor> into;
+    bool add = false;
+    c10::intrusive_ptr<GradHolder> holder;
+    if (need_dw && ctx->saved_data.count("holder")) {
+      holder = c10::static_intrusive_pointer_cast<GradHolder>(ctx->saved_data["holder"].toCapsule());
+      pybind11::gil_scoped_acquire gil;
+      into = holder->obj.attr("buf").cast<at::Tensor>();
+      add = holder->obj.attr("ready").cast<bool>();
+    }
+    const at::Tensor &x = saved[0], &w = saved[1], &targets = saved[2], &status = saved[3], &a = saved[4], &b = saved[5];
+    auto got = kind == PIECE   ? linear_ce_bwd(x, w, targets, a, b, grad, need_dx, need_dw, into, add, status)
+               : kind == SCALE ? linear_ce_bwd_scale(a, b, grad, into, add)
+                               : linear_ce_bwd_again(x, w, targets, a, b, grad, need_dx, need_dw,
+                                                     ctx->saved_data["max_bytes"].toInt(), into, add, status);
+    if (holder) {
+      pybind11::gil_scoped_acquire gil;
+      holder->obj.attr("ready") = true;
+      got[1] = at::Tensor();
+    }
+    at::Tensor none;
+    return {got[0], got[1], none, none, none, none, none, none, none};
+  }
+};
+
+// Rows that a tensor map can describe: 2D, unit inner stride, 16-byte rows that do not overlap.
+at::Tensor as_rows(const at::Tensor& t) {
+  at::Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  const bool fits = r.stride(1) == 1 && r.stride(0) % 8 == 0 && r.stride(0) >= r.size(1) &&
+                    reinterpret_cast<uintptr_t>(r.const_data_ptr()) % 16 == 0;
+  return fits ? r : r.clone(at::MemoryFormat::Contiguous);
+}
+
+// The checks of ops/functional.py's plain path, for CUDA tensors; nothing for types and sizes that the kernels do not take.
+c10::optional<at::Tensor> linear_ce(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& targets, int64_t reduction,
+                                    int64_t max_bytes, const at::Tensor& status, const pybind11::object& holder) {
+  TORCH_CHECK_VALUE(weight.dim() == 2 && x.dim() >= 1 && x.size(-1) == weight.size(1), "x [..., H] and weight [V, H] do not match");
+  TORCH_CHECK_VALUE(targets.sizes() == x.sizes().slice(0, x.dim() - 1), "targets must have the shape of x without its last axis");
+  TORCH_CHECK_VALUE(at::isIntegralType(targets.scalar_type(), false), "targets must be integers");
+  TORCH_CHECK_VALUE(weight.numel() > 0, "weight is empty");
+  TORCH_CHECK_VALUE(x.device() == weight.device() && x.device() == targets.device(), "x, weight and targets are on different devices");
+  TORCH_CHECK_VALUE(max_bytes > 0, "max_workspace must be positive");
+  if (x.scalar_type() != at::kBFloat16 || weight.scalar_type() != at::kBFloat16 || weight.size(1) % 8) return c10::nullopt;
+  const at::Tensor x2 = as_rows(x), w = as_rows(weight);
+  const at::Tensor flat = (targets.dim() == 1 ? targets : targets.reshape({-1})).to(at::kLong).contiguous();
+  const bool grad = at::GradMode::is_enabled();
+  const bool need_dx = grad && x2.requires_grad(), need_dw = grad && w.requires_grad();
+  at::Tensor out;
+  if (need_dx || need_dw) {
+    c10::intrusive_ptr<GradHolder> h;
+    if (!holder.is_none() && weight.is_contiguous() && w.is_same(weight)) h = c10::make_intrusive<GradHolder>(holder);
+    out = LinearCE::apply(x2, w, flat, reduction, need_dx, need_dw, max_bytes, status, h);
+  } else {
+    Kept kept;
+    out = linear_ce_fwd(x2, w, flat, reduction, false, false, max_bytes, status, kept);
+  }
+  return reduction == NONE && targets.dim() != 1 ? out.view(targets.sizes()) : out;
+}
+
 }  // namespace
 
-void register_linear_ce(pybind11::module& m) {
-  m.def("linear_ce_fwd", &linear_ce_fwd);
-  m.def("linear_ce_bwd", &linear_ce_bwd);
-  m.def("linear_ce_bwd_scale", &linear_ce_bwd_scale);
-  m.def("linear_ce_bwd_again", &linear_ce_bwd_again);
-}
+void register_linear_ce(pybind11::module& m) { m.def("linear_ce", &linear_ce); }

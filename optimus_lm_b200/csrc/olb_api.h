@@ -112,10 +112,14 @@ typedef struct {
   long long ce_part_ld;
   int* ce_flags;
   int ce_repair;
+  int ce_overlap;            // the launch before this one on the stream is olb_lce_prep: start under it
+  int wide_tiles;            // DENSE: CTA-pair tiles also for an N below 2048 that is no multiple of 256, where they waste
+                             // at most an eighth of it
 } olb_gemm_desc;
 
 int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream);
-int olb_gemm_ce_block_n(int M, int N);
+// Columns of a statistics tile of the cross-entropy product; *pair (may be NULL): CTA pairs take 256 x 256 tiles.
+int olb_gemm_ce_block_n(int M, int N, int* pair);
 
 // ---------------------------------------------------------------- normalisation (norm.cu)
 // y = x * rsqrt(mean(x^2) + eps) * w   (w may be NULL).  rstd [rows] fp32 is saved for backward.
@@ -233,11 +237,12 @@ int olb_ce_partial_bwd(const void* logits, long long ldl, const long long* label
 // ---------------------------------------------------------------- cross entropy from hidden states (linear_ce.cu)
 // The passes around the OLB_EPI_CE product; `rows` is one piece of the batch (see linear_ce.cu for the formulas).
 // ref[r] = x_r . w_t (fp32) for rows with a target t in [0, V), else 0; zeroes ce_max [rows], ce_flags
-// [1 + ceil(rows / 128)] and *ticket.
+// [1 + ceil(rows / 128)] and *ticket.  With count: count[0] = number of all_targets [n_all] in [0, V) (as fp32, rounded
+// above 2^24), count[1] = 1 / that (0 when there are none).  A product launched next (OLB_EPI_CE, ce_overlap) may
+// start before this is done.
 int olb_lce_prep(const void* x, long long ldx, const void* w, long long ldw, const long long* targets, int rows, int H,
-                 int V, float* ref, unsigned* ce_max, int* ce_flags, unsigned* ticket, cudaStream_t stream);
-// *count = number of targets in [0, V) (as fp32; exact up to 2^24), *inv_count = 1 / *count (0 when there are none).
-int olb_lce_count(const long long* targets, long long n, int V, float* count, float* inv_count, cudaStream_t stream);
+                 int V, float* ref, unsigned* ce_max, int* ce_flags, unsigned* ticket, const long long* all_targets,
+                 long long n_all, float* count, cudaStream_t stream);
 // Sums ce_part over its `ntiles` tiles and writes per row loss[r] (0 without a target) and, when they are not NULL,
 // prob[r] = 1 - p_target, lse[r], and with E (the exponentials, row stride lde): the target's entry of E, and
 // factor[r] such that factor[r] * E[r, :] is the row's gradient (times *scale when scale is not NULL); xs (may be NULL):

@@ -61,6 +61,9 @@ __device__ __forceinline__ bool elect_one() {
   return pred != 0;
 }
 
+// Until the launch before this one on the stream (programmatic dependent launch) has finished and its writes are visible.
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ------------------------------------------------------------------ mbarrier
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");

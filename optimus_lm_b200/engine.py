@@ -72,6 +72,8 @@ class EngineArgs:
     force_uniform_routing: bool = False
     use_local_router_aux_loss: bool = False
     use_fused_ep_alltoall: bool = True
+    use_linear_cross_entropy: bool = False  # loss straight from the hidden states, without logits (no pipeline stages, no TP)
+    opt_use_list_clipping: bool = False     # optimizer "pt": norm and clipping over all gradients in one call, fp32 norm
     skip_optimizer_step: bool = False
     skip_optimizer_step_weight_update: bool = False
     skip_backward_pass: bool = False
@@ -89,12 +91,13 @@ class StepOutput:
 
 
 def build_model(model_choice: str, pmap, *, dtype=torch.bfloat16, device="cpu", memory_tracker=None,
-                config_overrides=None, **parallel_kwargs):
+                config_overrides=None, use_linear_cross_entropy=False, **parallel_kwargs):
     """Construct (config, model) for ``model_choice`` on ``device`` with uninitialised weights."""
     cfg = config_utils.build_config(model_choice, **parallel_kwargs)
     for k, v in (config_overrides or {}).items():
         setattr(cfg, k, v)
     cfg.check_compatibility()
+    cfg.use_linear_cross_entropy = use_linear_cross_entropy or getattr(cfg, "use_linear_cross_entropy", False)
     fam = config_utils.model_family(model_choice)
     if fam == "olmoe":
         from .models.olmoe.modeling_olmoe import OlmoeParallelForCausalLM as M
@@ -214,7 +217,7 @@ class TrainEngine:
         if model is None:
             config, model = build_model(
                 args.model_choice, pmap, dtype=self.dtype, device=self.device,
-                config_overrides=args.config_overrides,
+                config_overrides=args.config_overrides, use_linear_cross_entropy=args.use_linear_cross_entropy,
                 pipeline_parallelism=args.pipeline_parallelism, expert_parallelism=args.expert_parallelism,
                 tensor_parallelism=args.tensor_parallelism,
                 virtual_pipeline_parallelism=args.virtual_pipeline_parallelism,
@@ -245,6 +248,8 @@ class TrainEngine:
                       expert_parallelism=p.expert_parallelism, ep_ind=p.ep_ind, ep_group=p.ep_group,
                       dpep_ind=p.dpep_ind, dpep_group=p.dpep_group, skip_optimizer_step=a.skip_optimizer_step,
                       opt_use_chunked_allreduce=a.opt_use_chunked_allreduce)
+        if a.optimizer == "pt":
+            kwargs.update(opt_use_list_clipping=a.opt_use_list_clipping)
         if a.optimizer not in ("unsharded", "pt"):
             kwargs.update(opt_use_allreduce_for_grad_acc=a.opt_use_allreduce_for_grad_acc,
                           opt_use_allreduce_for_param_gather=a.opt_use_allreduce_for_param_gather,

@@ -301,6 +301,8 @@ class ParallelDenseForCausalLM(nn.Module):
         else:
             self.lm_head = nn.Identity()
         self.inplace_ce_backward = True
+        # the tensor-parallel head splits the hidden dimension: its logits are partial sums and must exist
+        self.use_linear_cross_entropy = getattr(config, "use_linear_cross_entropy", False) and pmap.tensor_parallelism == 1
 
     def loss_function(self, logits, labels, vocab_size=None):
         return OF.shifted_cross_entropy(logits, labels, inplace_backward=self.inplace_ce_backward)
@@ -318,6 +320,9 @@ class ParallelDenseForCausalLM(nn.Module):
         output_stage = self.pmap.is_last_stage_rank and vp_ind == VPP - 1
         if PP > 1 and not output_stage:
             return {"output": hidden_states, "router_logits": None} if self.pp_dict_outputs else hidden_states
+        if PP == 1 and labels is not None and self.use_linear_cross_entropy:
+            loss = OF.shifted_linear_cross_entropy(hidden_states, self.lm_head.weight, labels)   # no logits
+            return self.output_class(loss=loss, logits=None)
         logits = self._head(hidden_states)
         if PP > 1:
             return {"output": logits, "router_logits": None} if self.pp_dict_outputs else logits

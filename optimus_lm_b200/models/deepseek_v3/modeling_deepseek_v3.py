@@ -442,6 +442,7 @@ class DeepseekV3ParallelForCausalLM(nn.Module):
         self.lm_head = (nn.Linear(config.hidden_size, config.vocab_size, bias=False)
                         if pmap.is_last_stage_rank else nn.Identity())
         self.inplace_ce_backward = True
+        self.use_linear_cross_entropy = getattr(config, "use_linear_cross_entropy", False)
 
     def loss_function(self, logits, labels, vocab_size=None):
         return OF.shifted_cross_entropy(logits, labels, inplace_backward=self.inplace_ce_backward)
@@ -451,10 +452,14 @@ class DeepseekV3ParallelForCausalLM(nn.Module):
         PP = self.pmap.pipeline_parallelism
         if PP > 1 and not self.pmap.is_last_stage_rank:
             return {"output": hidden_states, "router_logits": None}
-        logits = OF.linear(hidden_states, self.lm_head.weight)
-        if PP > 1:
-            return {"output": logits, "router_logits": None}
-        loss = self.loss_function(logits, labels, self.vocab_size) if labels is not None else None
+        logits = None
+        if PP == 1 and labels is not None and self.use_linear_cross_entropy:
+            loss = OF.shifted_linear_cross_entropy(hidden_states, self.lm_head.weight, labels)   # no logits
+        else:
+            logits = OF.linear(hidden_states, self.lm_head.weight)
+            if PP > 1:
+                return {"output": logits, "router_logits": None}
+            loss = self.loss_function(logits, labels, self.vocab_size) if labels is not None else None
         if self.training and getattr(self.config, "update_router_bias", False):
             for layer in self.model.layers:
                 if isinstance(layer.mlp, DeepseekV3ParallelMoE):

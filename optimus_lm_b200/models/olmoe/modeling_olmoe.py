@@ -240,6 +240,7 @@ class OlmoeParallelForCausalLM(nn.Module):
         self.use_local_router_aux_loss = config.use_local_router_aux_loss
         self.VPP = getattr(config, "virtual_pipeline_parallelism", 1)
         self.inplace_ce_backward = True
+        self.use_linear_cross_entropy = getattr(config, "use_linear_cross_entropy", False)
 
     def loss_function(self, logits, labels, vocab_size=None):
         return OF.shifted_cross_entropy(logits, labels, inplace_backward=self.inplace_ce_backward)
@@ -270,13 +271,15 @@ class OlmoeParallelForCausalLM(nn.Module):
             return self.lm_head(hidden_states) if is_output_stage else hidden_states
         if PP > 1 and not self.pmap.is_last_stage_rank:
             return {"output": hidden_states, "router_logits": router_logits}
-        logits = OF.linear(hidden_states, self.lm_head.weight)
-        if PP > 1:
-            return {"output": logits, "router_logits": router_logits}
-
-        loss = None
-        if labels is not None:
-            loss = self.loss_function(logits, labels, self.vocab_size)
+        loss = logits = None
+        if PP == 1 and labels is not None and self.use_linear_cross_entropy:
+            loss = OF.shifted_linear_cross_entropy(hidden_states, self.lm_head.weight, labels)   # no logits
+        else:
+            logits = OF.linear(hidden_states, self.lm_head.weight)
+            if PP > 1:
+                return {"output": logits, "router_logits": router_logits}
+            if labels is not None:
+                loss = self.loss_function(logits, labels, self.vocab_size)
         aux_loss = None
         if self.output_router_logits:
             aux_loss = self.aux_loss_from_router(router_logits, self.model.layers)

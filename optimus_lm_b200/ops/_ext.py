@@ -63,7 +63,7 @@ def use_kernels(*tensors: torch.Tensor) -> bool:
 # Kernel launches issued per binding call (see csrc/*.cu launchers).
 _LAUNCHES_PER_CALL = {
     "moe_build_index": 4, "sumsq": 2, "attn_bwd": 3,
-    "linear_ce_fwd": 5, "linear_ce_bwd": 3, "linear_ce_bwd_scale": 2, "linear_ce_bwd_again": 6,  # of one piece
+    "linear_ce": 5,  # the forward of one piece; its backward's three do not pass through here
     "grad_clip": 2,
 }
 

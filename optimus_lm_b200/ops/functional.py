@@ -965,48 +965,6 @@ def linear_cross_entropy_reference(x, weight, targets, reduction="mean"):
     return loss.view(targets.shape) if reduction == "none" else loss
 
 
-class _LinearCEFn(torch.autograd.Function):
-    """See csrc/linear_ce_bindings.cpp for what forward leaves to backward.  The last two tensors it returns depend on
-    whether the batch fitted one piece: exponentials and row factors, finished gradients, or per-row statistics."""
-
-    @staticmethod
-    def forward(ctx, x2, w, targets, reduction, holder, max_workspace):
-        need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        out, a, b = extension().linear_ce_fwd(x2, w, targets, _LCE_REDUCTIONS[reduction], need_dx, need_dw, max_workspace,
-                                              status_word(x2.device))
-        if a is not None and a.dtype == torch.bfloat16 and a.shape[0] >= x2.shape[0] and b is not None and b.dim() == 1:
-            ctx.kind = "piece"
-        elif reduction == "none":
-            ctx.kind = "again"
-        else:
-            ctx.kind = "scale"
-        ctx.save_for_backward(x2, w, targets, a, b)
-        ctx.misc = (reduction, holder, max_workspace)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        x2, w, targets, a, b = ctx.saved_tensors
-        reduction, h, max_workspace = ctx.misc
-        need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        grad = grad.to(torch.float32).contiguous()
-        C = extension()
-        direct = h is not None and need_dw
-        out, add = (h.buf, h.ready) if direct else (None, False)
-        if ctx.kind == "piece":
-            dx, dw = C.linear_ce_bwd(x2, w, targets, a, b, grad, need_dx, need_dw, out, add, status_word(x2.device))
-        elif ctx.kind == "scale":
-            dx, dw = C.linear_ce_bwd_scale(a, b, grad, out, add)
-        else:
-            dx, dw = C.linear_ce_bwd_again(x2, w, targets, a, b, grad, need_dx, need_dw, max_workspace, out, add,
-                                           status_word(x2.device))
-        if direct:
-            h.ready = True
-            dw = None
-        return dx, dw, None, None, None, None
-
-
 def linear_cross_entropy(x, weight, targets, reduction="mean", max_workspace=1 << 30):
     """Cross entropy of ``softmax(x @ weight.T)`` against ``targets`` without the logits in memory.
 
@@ -1022,34 +980,30 @@ def linear_cross_entropy(x, weight, targets, reduction="mean", max_workspace=1 <
 
     The kernel path takes bf16 CUDA tensors with ``H % 8 == 0``; other inputs take the plain one.  Reference: the
     ``lm_head`` of optimus/models/olmoe/modeling_olmoe.py:502-524 and ``F.cross_entropy`` on its logits."""
-    if reduction not in _LCE_REDUCTIONS:
+    code = _LCE_REDUCTIONS.get(reduction)
+    if code is None:
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', not {reduction!r}")
+    lazy = getattr(weight, "_olb_lazy", None)
+    if lazy is not None and lazy.stale:
+        lazy.materialize(weight)
+    if x.is_cuda and use_kernels(x):
+        out = extension().linear_ce(x, weight, targets, code, int(max_workspace), status_word(x.device), _holder(weight))
+        if out is not None:
+            return out
+    # the same refusals for the plain path
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"x [..., H] and weight [V, H] do not match: {tuple(x.shape)}, {tuple(weight.shape)}")
     if targets.shape != x.shape[:-1]:
         raise ValueError(f"targets {tuple(targets.shape)} must have the shape of x without its last axis {tuple(x.shape)}")
     if targets.is_floating_point() or targets.is_complex() or targets.dtype == torch.bool:
         raise ValueError(f"targets must be integers, not {targets.dtype}")
-    if weight.shape[0] == 0 or weight.shape[1] == 0:
+    if weight.numel() == 0:
         raise ValueError("weight is empty")
     if not (x.device == weight.device == targets.device):
         raise ValueError(f"x, weight and targets are on different devices: {x.device}, {weight.device}, {targets.device}")
     if max_workspace <= 0:
         raise ValueError("max_workspace must be positive")
-    lazy = getattr(weight, "_olb_lazy", None)
-    if lazy is not None and lazy.stale:
-        lazy.materialize(weight)
-    if not (_kernel_ok(x, weight) and weight.shape[1] % 8 == 0):
-        return linear_cross_entropy_reference(x, weight, targets, reduction)
-    x2 = _as_2d(x)
-    w = _as_2d(weight)
-    flat = targets.reshape(-1).to(torch.long).contiguous()
-    if torch.is_grad_enabled() and (x2.requires_grad or w.requires_grad):
-        out = _LinearCEFn.apply(x2, w, flat, reduction, _holder(weight) if weight.is_contiguous() and weight.data_ptr() % 16 == 0 else None, int(max_workspace))
-    else:
-        out = extension().linear_ce_fwd(x2, w, flat, _LCE_REDUCTIONS[reduction], False, False, int(max_workspace),
-                                        status_word(x2.device))[0]
-    return out.view(targets.shape) if reduction == "none" else out
+    return linear_cross_entropy_reference(x, weight, targets, reduction)
 
 
 def shifted_linear_cross_entropy(hidden, weight, labels):

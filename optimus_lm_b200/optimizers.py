@@ -749,11 +749,13 @@ class TorchAdamW:
     data-parallel replicas; here the gradients are averaged over the data-parallel group right before the
     update, which gives the same numbers without a wrapper module around the model.  Gradient clipping to norm 1
     starts after ``warmup_steps`` optimizer steps unless delayed clipping is disabled, with the local norm as in the
-    reference.  Takes the constructor keywords of the flat-buffer classes and ignores those it has no use for."""
+    reference.  ``opt_use_list_clipping`` takes norm and clipping through ``ops.functional.grad_norm`` and
+    ``clip_grad_norm_``: one call over all gradients and an fp32 norm, where torch's utilities launch kernels per
+    tensor and give bf16 gradients a bf16 norm.  Takes the constructor keywords of the flat-buffer classes and ignores those it has no use for."""
 
     def __init__(self, params, model, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, warmup_steps=0,
                  num_shards=1, group=None, opt_disable_delayed_grad_clipping=False, skip_optimizer_step=False,
-                 opt_use_one_step_grad_clipping=False, **_unused):
+                 opt_use_one_step_grad_clipping=False, opt_use_list_clipping=False, **_unused):
         self.model = model
         self.inner = torch.optim.AdamW(list(params), lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
         self.param_groups = self.inner.param_groups
@@ -763,6 +765,7 @@ class TorchAdamW:
         self.opt_disable_delayed_grad_clipping = opt_disable_delayed_grad_clipping
         self.skip_optimizer_step = skip_optimizer_step
         self.one_step_clipping = opt_use_one_step_grad_clipping
+        self.list_clipping = opt_use_list_clipping
         self.max_grad_norm = 1.0
         self.step_id = 0
 
@@ -777,9 +780,13 @@ class TorchAdamW:
                 dist.all_reduce(p.grad, group=self.group)
                 p.grad.div_(self.num_shards)
         grads = [p.grad for p in ps]
-        grad_norm = torch.nn.utils.get_total_norm(grads) if grads else torch.zeros(())
-        if grads and (self.opt_disable_delayed_grad_clipping or self.step_id >= self.warmup_steps):
-            torch.nn.utils.clip_grads_with_norm_(ps, self.max_grad_norm, grad_norm)
+        clip = bool(grads) and (self.opt_disable_delayed_grad_clipping or self.step_id >= self.warmup_steps)
+        if self.list_clipping:
+            grad_norm = OF.clip_grad_norm_(grads, self.max_grad_norm) if clip else OF.grad_norm(grads)
+        else:
+            grad_norm = torch.nn.utils.get_total_norm(grads) if grads else torch.zeros(())
+            if clip:
+                torch.nn.utils.clip_grads_with_norm_(ps, self.max_grad_norm, grad_norm)
         if not self.skip_optimizer_step:
             self.inner.step()
         self.step_id += 1

@@ -70,6 +70,8 @@ LISTS = {
     "with empty ones": [0, 5, 0, 0, 70000, 0],
     "small table full": [11] * 250,
     "one more": [11] * 251,
+    "middle table full": [9] * 800,
+    "and one more": [9] * 801,
     "large table full": [3] * 2040,
     "one more than that": [3] * 2041,
     "thousands": [1 + (k * 37) % 400 for k in range(5000)],

@@ -327,3 +327,31 @@ def test_streams_and_capture():
         for (loss, dx, dw), kw in zip(outs, ({}, {"max_workspace": 1})):
             for a, b in zip((loss, dx, dw), run_both(x2, w2, t2, "mean", **kw)):
                 assert torch.equal(a, b)
+
+
+def test_refusals():
+    x, w, t = make(37, 16, 50)
+    ok = dict(x=x, weight=w, targets=t)
+    for change in (dict(reduction="median"), dict(weight=w[:, :8]), dict(weight=w[0]), dict(targets=t[:-1]), dict(targets=t.float()),
+                   dict(targets=t > 3), dict(weight=w[:0]), dict(targets=t.view(1, -1)), dict(max_workspace=0),
+                   dict(targets=t.cpu()), dict(weight=w.cpu())):
+        with pytest.raises(ValueError):
+            OF.linear_cross_entropy(**{**ok, **change})
+    # what the kernels do not take goes the plain way
+    for a, b in ((x.float(), w.float()), (x, w.float()), (x[:, :12], w[:, :12])):
+        assert torch.isfinite(OF.linear_cross_entropy(a, b, t))
+
+
+def test_once_differentiable():
+    x, w, t = make(37, 16, 50)
+    x.requires_grad_()
+    loss = OF.linear_cross_entropy(x, w, t)
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(loss, x, create_graph=True)
+
+
+def test_many_rows_and_few_columns():
+    # row blocks past the first band of tiles, and a vocabulary below one tile
+    x, w, t = make(5000, 64, 50, seed=31, ignored=0.1)
+    check(x, w, t, "mean")
+    check(x, w, t, "none", max_workspace=1 << 18)
