@@ -95,6 +95,8 @@ struct GemmParams {
   long long ce_part_ld;
   int* ce_flags;               // [0] any row block flagged, [1 + b] row block b (128 rows) flagged
   float ce_grow;               // see epilogue_ce
+  int ce_a_rows;               // rows of A in a tile's boxes: 128, or fewer in a launch of one row block
+  int ce_tile_n;               // columns per tile, a multiple of 32 up to BLOCK_N
   int ce_overlap;              // the launch before this one may still be running: wait for it before its results are read
   int ce_repair;               // only the flagged row blocks, with their rows' recorded maxima as references
   int ce_store;                // the exponentials are written to C
@@ -156,6 +158,9 @@ __device__ __forceinline__ int stale_vectors_in_block(const PeerArg<true>& peers
 }
 constexpr int STAGER_WARPS = 4;
 constexpr int NUM_THREADS_STAGED = NUM_THREADS + 32 * STAGER_WARPS;
+// Epilogue warps of a CTA and threads of a launch (EPI_CE: sixteen, see epilogue_ce).
+__host__ __device__ constexpr int epilogue_warps(int epi) { return epi == 4 ? 16 : 4; }
+__host__ __device__ constexpr int num_threads(bool peer, int epi) { return peer ? NUM_THREADS_STAGED : 64 + 32 * epilogue_warps(epi); }
 
 // Epilogue staging: each of the four epilogue warps owns two buffers of 32 rows x 128 bytes (what one tensor-map
 // store of its rows takes), laid out with the 128-byte swizzle the store expects.
@@ -191,7 +196,7 @@ __device__ __forceinline__ void set_k_range(const GemmParams& p, int part, TileI
 // Map a linear tile id to its coordinates.  Returns false when `t` is past the last tile.
 template <int BLOCK_N, int EPI = EPI_PLAIN>
 __device__ __forceinline__ bool get_tile(const GemmParams& p, int t, int num_m_blocks, int blk0, TileInfo& ti) {
-  constexpr int TILE_N = EPI == EPI_SWIGLU ? BLOCK_N / 2 : BLOCK_N;  // output columns per tile
+  const int TILE_N = EPI == EPI_SWIGLU ? BLOCK_N / 2 : (EPI == EPI_CE ? p.ce_tile_n : BLOCK_N);  // output columns per tile
   const int num_n_blocks = (p.N + TILE_N - 1) / TILE_N;
   if (p.mode == OLB_GEMM_RAGGED_K) {
     const int per_expert = num_m_blocks * num_n_blocks;
@@ -560,72 +565,125 @@ __device__ __forceinline__ bool ce_skip_tile(const GemmParams& p, const TileInfo
 
 // Epilogue of one 128-row tile of the cross-entropy product: the accumulator holds the logits l of the row against
 // vocabulary columns [ti.n0, ti.n0 + BLOCK_N).  With the row's reference m (its target's logit, or a log-sum-exp that
-// is known already) it writes e = exp(l - m) as bf16 to C (ce_store) and the row's sum of e over the tile without
-// the target's column to ce_part[column tile][row].  exp is taken of the fp32 difference: nothing is rounded to fewer
-// bits before it, and e keeps bf16's relative precision however small it is.  Columns past N and rows without a target
-// give zeros.  A row whose logits exceed the reference by more than CE_RANGE has its largest logit recorded in ce_max
-// and its row block flagged; a second launch (ce_repair) computes those blocks again against the recorded maxima.
+// is known already) it writes e = exp(l - m) as bf16 to C (ce_store) and the row's sum of e over half a tile without
+// the target's column to ce_part[half tile][row].  exp is taken of fp32 values as 2^(l c - m log2e), one multiply-add
+// and one exponential for a logit; the rounding of m log2e is common to a row and goes back into its sum.  Nothing is
+// rounded to fewer bits before that, and e keeps bf16's relative precision however small it is.  Columns past N and
+// rows without a target give zeros.  A row whose sum shows a logit more than CE_RANGE above the reference has its
+// largest logit recorded in ce_max and its row block flagged; a second launch (ce_repair) computes those blocks again
+// against the recorded maxima.
 // The tensor cores truncate as they add: against the exact sum a logit of H terms of random sign comes out smaller by
 // 1.4e-8 of itself for every 16 terms (measured: 4.0e-7 at H = 512, 1.8e-6 at 2048, 6.9e-6 at 7168; up to 6e-8 where all
-// terms have one sign), and a mean loss would keep that bias.  ce_grow = 1 + 1.4e-8 H / 16 gives it back in the
-// multiply-add that takes the difference, which halves the logits' rms error (2.1e-6 to 1.1e-6 at H = 2048).
+// terms have one sign), and a mean loss would keep that bias.  c = ce_grow = log2e (1 + 1.4e-8 H / 16) gives it back,
+// which halves the logits' rms error (2.1e-6 to 1.1e-6 at H = 2048).
 // CE_RANGE: sums of 2^31 terms of e^40 = 2.4e17 stay below 1e27, far inside fp32 and bf16, and so does their inverse.
-constexpr float CE_RANGE = 40.f;
+//
+// Sixteen warps per CTA work on a tile: each four take a quarter of its columns (a warp's dependent instructions leave
+// a scheduler idle three cycles of four: 3000 x 64 against 30000 took 88 us with four warps, 70 with eight).  A chunk of
+// 32 rows x 32 columns goes through a swizzled 2 KB of shared memory and out with plain 16-byte stores of whole sectors:
+// bulk stores, two in flight per warp, took as long again as the arithmetic.
+constexpr float CE_RANGE_SUM = 2.3538527e17f;  // e^40
 template <int BLOCK_N>
-__device__ __forceinline__ void epilogue_ce(const GemmParams& p, const CUtensorMap* tma_c, EpiStage& es, uint32_t taddr,
-                                            const TileInfo& ti, int lane_group, int lane) {
-  const int row = ti.m0 + lane_group * 32 + lane;
-  const int y = ti.m0 + lane_group * 32;
-  if (y >= p.M) return;
+__device__ __forceinline__ void epilogue_ce(const GemmParams& p, uint32_t stage, uint32_t taddr, const TileInfo& ti,
+                                            int lane_group, int part, int lane) {
+  constexpr int COLS = BLOCK_N / 4;                 // columns of this warp, fewer at the end of a narrower tile
+  constexpr int CHUNK = COLS < 32 ? COLS : 32;      // columns per turn
+  constexpr int UNITS = CHUNK / 8, ROWS = 32 / UNITS;  // 16-byte units of a row, rows written per turn of the warp
+  const int row0 = ti.m0 + lane_group * 32, row = row0 + lane;
+  const int x0 = ti.n0 + part * COLS;
+  const int x_end = min(p.N, ti.n0 + p.ce_tile_n);
+  if (row0 >= p.M || x0 >= x_end) return;
   const bool row_ok = row < p.M;
   const long long target = row_ok ? p.ce_targets[row] : -1;
   const bool live = target >= 0 && target < p.N;
-  const int tcol = live ? static_cast<int>(target) - ti.n0 : -1;
+  const bool all_live = __all_sync(0xffffffffu, live);
+  const int tcol = live ? static_cast<int>(target) - x0 : -1;
+  constexpr float LOG2E = 1.4426950408889634f;
   const float ref = live ? ce_row_ref(p, row) : 0.f;
-  const float2 neg_ref = make_float2(-ref, -ref);
+  const float ref2 = ref * LOG2E;
+  // 2^(ref2 - ref log2e), to be given back: the product's rounding and that of the constant (LOG2E = log2e + 1.9e-8 log2e)
+  const float slip = (fmaf(-ref, LOG2E, ref2) + ref * 2.7e-8f) * 0.6931472f;
+  const float2 neg_ref2 = make_float2(-ref2, -ref2);
   const float2 grow = make_float2(p.ce_grow, p.ce_grow);
-  const float2 log2e = make_float2(1.4426950408889634f, 1.4426950408889634f);
-  float top = -INFINITY;
+  const uint32_t cols = taddr + part * COLS;
   float2 sum = make_float2(0.f, 0.f);
+  // this lane's part of the coalesced stores: rows lane / UNITS + k * ROWS, 16-byte unit lane % UNITS
+  const uint32_t st_row = stage + lane * (UNITS * 16);
+  const int ld_r = lane / UNITS, ld_u = lane % UNITS;
+  constexpr int SPREAD = 8 / UNITS;  // rows in 128 bytes of the buffer
+  char* out = static_cast<char*>(p.C) + (static_cast<long long>(row0 + ld_r) * p.ldc + x0 + ld_u * 8) * 2;
+  const long long out_step = static_cast<long long>(ROWS) * p.ldc * 2;
+  const int rows_left = p.M - row0 - ld_r;
 #pragma unroll 1
-  for (int c = 0; c < BLOCK_N / 64; ++c) {
-    const int x = ti.n0 + c * 64;
-    if (x >= p.N) break;
-    uint32_t r[64], v[32];
-    tmem_ld_32x32b_x32(taddr + c * 64, *reinterpret_cast<uint32_t(*)[32]>(r));
-    tmem_ld_32x32b_x32(taddr + c * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(r + 32));
+  for (int c = 0; c < COLS / CHUNK; ++c) {
+    const int x = x0 + c * CHUNK;
+    if (x >= x_end) break;
+    uint32_t r[CHUNK], v[CHUNK / 2];
+    if constexpr (CHUNK == 32) tmem_ld_32x32b_x32(cols + c * CHUNK, r);
+    else tmem_ld_32x32b_x16(cols + c * CHUNK, r);
     tmem_ld_wait();
-    if (x + 64 > p.N) {
+    if (x + CHUNK > p.N) {
 #pragma unroll
-      for (int i = 0; i < 64; ++i)
+      for (int i = 0; i < CHUNK; ++i)
         if (x + i >= p.N) r[i] = 0xff800000u;  // -inf: e = 0
     }
-    const int tc = tcol - c * 64;
-    const bool here = tc >= 0 && tc < 64;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const float2 l = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-      top = max3(top, l.x, l.y);
-      const float2 d = mul2(fma2(l, grow, neg_ref), log2e);
+    for (int i = 0; i < CHUNK / 2; ++i) {
+      const float2 d = fma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), grow, neg_ref2);
       r[2 * i] = __float_as_uint(ex2_approx(d.x));
       r[2 * i + 1] = __float_as_uint(ex2_approx(d.y));
     }
-    if (__any_sync(0xffffffffu, here)) {
+    const int tc = tcol - c * CHUNK;
+    if (__any_sync(0xffffffffu, tc >= 0 && tc < CHUNK)) {
 #pragma unroll
-      for (int i = 0; i < 64; ++i)
+      for (int i = 0; i < CHUNK; ++i)
         if (i == tc) r[i] = 0u;
     }
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < CHUNK / 2; ++i) {
       const float2 e = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
       sum = add2(sum, e);
-      v[i] = live ? pack_bf16(e.x, e.y) : 0u;
+      v[i] = pack_bf16(e.x, e.y);
     }
-    if (p.ce_store) epi_store_chunk(es, tma_c, v, lane, x, y);
+    if (p.ce_store) {
+      if (!all_live && !live) {  // whatever such a row holds
+#pragma unroll
+        for (int i = 0; i < CHUNK / 2; ++i) v[i] = 0u;
+      }
+      // unit j of the lane's row goes to j ^ (row / SPREAD) % UNITS; then UNITS lanes write a row, ROWS rows a turn
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < UNITS; ++j)
+        st_shared_v4(st_row + ((j ^ ((lane / SPREAD) & (UNITS - 1))) << 4), v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      __syncwarp();
+      char* o = out + c * (CHUNK * 2);
+#pragma unroll
+      for (int j = 0; j < UNITS; ++j) {
+        const int rr = j * ROWS + ld_r;
+        const uint4 u = ld_shared_v4(stage + rr * (UNITS * 16) + ((ld_u ^ ((rr / SPREAD) & (UNITS - 1))) << 4));
+        if (j * ROWS < rows_left) *reinterpret_cast<uint4*>(o) = u;
+        o += out_step;
+      }
+    }
   }
-  if (!live) return;
-  if (p.ce_part) p.ce_part[static_cast<long long>(ti.n0 / BLOCK_N) * p.ce_part_ld + row] = sum.x + sum.y;
-  if (p.ce_flags && !p.ce_repair && top - ref > CE_RANGE) {
+  const float total = (sum.x + sum.y) * (1.f + slip);
+  const int slice = ti.n0 / p.ce_tile_n * ((p.ce_tile_n + COLS - 1) / COLS) + part;
+  if (live && p.ce_part) p.ce_part[static_cast<long long>(slice) * p.ce_part_ld + row] = total;
+  if (p.ce_flags == nullptr || p.ce_repair) return;
+  const bool far = live && !(total <= CE_RANGE_SUM);
+  if (!__any_sync(0xffffffffu, far)) return;
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < COLS / 16; ++c) {
+    if (x0 + c * 16 >= x_end) break;
+    uint32_t r[16];
+    tmem_ld_32x32b_x16(cols + c * 16, r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (x0 + c * 16 + i < x_end) top = fmaxf(top, __uint_as_float(r[i]));
+  }
+  if (far) {
     atomicMax(p.ce_max + row, ce_encode_max(top));
     p.ce_flags[1 + row / BLOCK_M] = 1;
     p.ce_flags[0] = 1;
@@ -787,7 +845,7 @@ __device__ __forceinline__ void stager_loop(const PeerArg<true>& peers, const Ge
 }
 
 template <int BLOCK_N, bool PEER, int EPI>
-__global__ void __launch_bounds__(PEER ? NUM_THREADS_STAGED : NUM_THREADS, 1)
+__global__ void __launch_bounds__(num_threads(PEER, EPI), 1)
 gemm_bf16_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                  const __grid_constant__ CUtensorMap tma_b2, const __grid_constant__ CUtensorMap tma_c,
                  const __grid_constant__ CUtensorMap tma_c2, const __grid_constant__ PeerArg<PEER> peers,
@@ -823,7 +881,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(acc_full_bar(a), 1);
-      mbar_init(acc_empty_bar(a), 4);
+      mbar_init(acc_empty_bar(a), epilogue_warps(EPI));
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -889,8 +947,13 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
           const uint32_t sa = smem_base + stage * L::STAGE_BYTES;
           const uint32_t sb = sa + A_STAGE_BYTES;
           const uint32_t fb = full_bar(stage);
-          mbar_expect_tx(fb, L::STAGE_BYTES);
-          const int k0 = kb * BLOCK_K;
+          mbar_expect_tx(fb, EPI == EPI_CE ? (p.ce_a_rows + p.ce_tile_n) * BLOCK_K * 2 : L::STAGE_BYTES);
+          int k0 = kb * BLOCK_K;
+          if constexpr (EPI == EPI_CE) {
+            // one row block: every CTA reads the same few lines of A, so each starts somewhere else in K (all CTAs on the
+            // same line at a time: 243 us for one row against 128256 x 4096, 186 us for 64 rows)
+            if (num_m_blocks == 1) k0 = ((kb + static_cast<int>(blockIdx.x) * ti.kb_end / static_cast<int>(gridDim.x)) % ti.kb_end) * BLOCK_K;
+          }
           if (!p.a_mn_major) {
             tma_load_2d(sa, &tma_a, fb, k0, ti.m0);
           } else {
@@ -936,7 +999,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (elect_one()) {
-      const uint32_t idesc = make_idesc_bf16(BLOCK_M, BLOCK_N, p.a_mn_major, p.b_mn_major);
+      const uint32_t idesc = make_idesc_bf16(BLOCK_M, EPI == EPI_CE ? p.ce_tile_n : BLOCK_N, p.a_mn_major, p.b_mn_major);
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
@@ -981,7 +1044,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
         }
       }
     }
-  } else if (warp < 6) {
+  } else if (warp < 2 + epilogue_warps(EPI)) {
     // ------------------------------------------------------------ epilogue (warps 2..5)
     if constexpr (EPI == EPI_CE) {
       if (p.ce_overlap) grid_dependency_wait();
@@ -1006,7 +1069,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
       if constexpr (EPI == EPI_SWIGLU) {
         epilogue_swiglu(p, &tma_c, &tma_c2, es, taddr, ti, lane_group, lane);
       } else if constexpr (EPI == EPI_CE) {
-        epilogue_ce<BLOCK_N>(p, &tma_c, es, taddr, ti, lane_group, lane);
+        epilogue_ce<BLOCK_N>(p, smem_base + L::EPI_OFFSET + (warp - 2) * (EPI_BUF_BYTES / 2), taddr, ti, lane_group, (warp - 2) >> 2, lane);
       } else {
         epilogue_plain<BLOCK_N, EPI == EPI_ROWSCALE>(p, &tma_c, es, taddr, ti, has_k, lane_group, lane);
       }
@@ -1105,7 +1168,7 @@ __device__ __forceinline__ bool get_tile_pair(const GemmParams& p, int t, int nu
 }
 
 template <bool PEER, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PEER ? NUM_THREADS_STAGED : NUM_THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(num_threads(PEER, EPI), 1)
 gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                       const __grid_constant__ CUtensorMap tma_b2, const __grid_constant__ CUtensorMap tma_c,
                       const __grid_constant__ CUtensorMap tma_c2, const __grid_constant__ PeerArg<PEER> peers,
@@ -1142,7 +1205,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(acc_full_bar(a), 1);
-      mbar_init(acc_empty_bar(a), 8);  // CTA 0's: four epilogue warps of each CTA
+      mbar_init(acc_empty_bar(a), 2 * epilogue_warps(EPI));  // CTA 0's: the epilogue warps of each CTA
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -1299,7 +1362,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
         }
       }
     }
-  } else if (warp < 6) {
+  } else if (warp < 2 + epilogue_warps(EPI)) {
     // ------------------------------------------------------------ epilogue (warps 2..5 of both CTAs, own 128 rows)
     if constexpr (EPI == EPI_CE) {
       if (p.ce_overlap) grid_dependency_wait();
@@ -1330,7 +1393,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
       } else if constexpr (EPI == EPI_SWIGLU_BWD) {
         epilogue_swiglu_bwd(p, &tma_c, es, taddr, mine, lane_group, lane);
       } else if constexpr (EPI == EPI_CE) {
-        epilogue_ce<BLOCK_N>(p, &tma_c, es, taddr, mine, lane_group, lane);
+        epilogue_ce<BLOCK_N>(p, smem_base + L::EPI_OFFSET + (warp - 2) * (EPI_BUF_BYTES / 2), taddr, mine, lane_group, (warp - 2) >> 2, lane);
       } else {
         epilogue_plain<BLOCK_N, EPI == EPI_ROWSCALE>(p, &tma_c, es, taddr, mine, has_k, lane_group, lane);
       }
@@ -1348,7 +1411,10 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
       if (has_k) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(acc ? acc_empty_remote1 : acc_empty_remote0);
+        if (lane == 0) {
+          if constexpr (EPI == EPI_CE) mbar_arrive_cluster_relaxed(acc ? acc_empty_remote1 : acc_empty_remote0);
+          else mbar_arrive_cluster(acc ? acc_empty_remote1 : acc_empty_remote0);
+        }
         if (++acc == 2) {
           acc = 0;
           acc_phase ^= 1u;
@@ -1502,16 +1568,16 @@ static int launch(const TensorMaps& tm, const PeerArg<PEER>& peers, const GemmPa
     if (e != cudaSuccess) return -3;
     configured[dev] = true;
   }
-  constexpr int TILE_N = EPI == EPI_SWIGLU ? BLOCK_N / 2 : BLOCK_N;
+  const int TILE_N = EPI == EPI_SWIGLU ? BLOCK_N / 2 : (EPI == EPI_CE ? p.ce_tile_n : BLOCK_N);
   const long long nm = (p.M + BLOCK_M - 1) / BLOCK_M, nn = (p.N + TILE_N - 1) / TILE_N;
   const long long tiles = nm * nn * (p.mode == OLB_GEMM_RAGGED_K ? p.num_experts : (p.k_splits > 1 ? p.k_splits : 1));
   int grid = static_cast<int>(tiles < num_sms ? tiles : num_sms);
   if (grid <= 0) return 0;
   if constexpr (EPI == EPI_CE) {
     if (p.ce_overlap)
-      return launch_overlapped(gemm_bf16_kernel<BLOCK_N, PEER, EPI>, grid, NUM_THREADS, L::TOTAL, stream, tm, peers, p);
+      return launch_overlapped(gemm_bf16_kernel<BLOCK_N, PEER, EPI>, grid, num_threads(PEER, EPI), L::TOTAL, stream, tm, peers, p);
   }
-  gemm_bf16_kernel<BLOCK_N, PEER, EPI><<<grid, PEER ? NUM_THREADS_STAGED : NUM_THREADS, L::TOTAL, stream>>>(
+  gemm_bf16_kernel<BLOCK_N, PEER, EPI><<<grid, num_threads(PEER, EPI), L::TOTAL, stream>>>(
       tm.a, tm.b, tm.b2, tm.c, tm.c2, peers, p);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
@@ -1538,9 +1604,9 @@ static int launch_pair(const TensorMaps& tm, const PeerArg<PEER>& peers, const G
   if (pairs <= 0) return 0;
   if constexpr (EPI == EPI_CE) {
     if (p.ce_overlap)
-      return launch_overlapped(gemm_bf16_pair_kernel<PEER, EPI>, 2 * pairs, NUM_THREADS, L::TOTAL, stream, tm, peers, p);
+      return launch_overlapped(gemm_bf16_pair_kernel<PEER, EPI>, 2 * pairs, num_threads(PEER, EPI), L::TOTAL, stream, tm, peers, p);
   }
-  gemm_bf16_pair_kernel<PEER, EPI><<<2 * pairs, PEER ? NUM_THREADS_STAGED : NUM_THREADS, L::TOTAL, stream>>>(
+  gemm_bf16_pair_kernel<PEER, EPI><<<2 * pairs, num_threads(PEER, EPI), L::TOTAL, stream>>>(
       tm.a, tm.b, tm.b2, tm.c, tm.c2, peers, p);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
@@ -1595,33 +1661,41 @@ static int device_sm_count() {
   return cached[dev];
 }
 
-}  // namespace olb
-
-// Tiles of the cross-entropy product: CTA pairs on 256 x 256, or one CTA on 128 x {256, 128, 64}, whichever takes the
-// fewest column-steps counted in whole waves over the SMs, with 32 columns for a tile's own start and end and 15 % for
-// what a single CTA loses against a pair.  So a short batch spreads the weight's rows over all SMs (one row against
-// 128256 x 4096: 195 us with 256 columns, four waves of 148 for 501 tiles) and a long one takes pairs.
-extern "C" int olb_gemm_ce_block_n(int M, int N, int* pair) {
-  using namespace olb;
+// Tiles of the cross-entropy product: CTA pairs on 256 x 256, or one CTA on 128 rows and 32 to 256 columns, whichever
+// takes the least time counted in whole waves over the SMs.  A tile's time goes with its columns (15 % more for what a
+// single CTA loses against a pair) or, narrow ones, with the rows of both operands that it loads, plus 32 columns for its
+// start and end.  So a short batch spreads the weight evenly over the SMs: one row against 128256 x 4096 takes 573 tiles
+// of 224 columns instead of 501 of 256, both in four waves of 148 (tiles of 128: 246 us, of 64: 412, of 256: 183).
+struct CePlan {
+  int block_n, tile_n, pair;
+};
+static CePlan ce_plan(int M, int N) {
   const long long sms = device_sm_count() > 1 ? device_sm_count() : 148;
   auto waves = [](long long tiles, long long workers) { return static_cast<double>((tiles + workers - 1) / workers); };
   const long long m = (M + 127) / 128;
-  int best = 256, with_pair = 0;
+  CePlan best{256, 256, 0};
   double least = 1e300;
   if (M >= 256 && pair_kernel_enabled()) {
     least = waves((M + 255) / 256 * ((N + 255ll) / 256), sms / 2) * (256 + 32);
-    with_pair = 1;
+    best.pair = 1;
   }
-  for (int bn : {256, 128, 64}) {
-    const double cost = waves(m * ((N + bn - 1ll) / bn), sms) * (1.15 * bn + 32);
+  for (int tn : {256, 224, 192, 160, 128, 96, 64, 32}) {
+    const double a_tile = 1.15 * tn > 0.75 * (128 + tn) ? 1.15 * tn : 0.75 * (128 + tn);
+    const double cost = waves(m * ((N + tn - 1ll) / tn), sms) * (a_tile + 32);
     if (cost < least) {
       least = cost;
-      best = bn;
-      with_pair = 0;
+      best = {tn > 128 ? 256 : (tn > 64 ? 128 : 64), tn, 0};
     }
   }
-  if (pair) *pair = with_pair;
   return best;
+}
+
+}  // namespace olb
+
+extern "C" int olb_gemm_ce_slices(int M, int N) {
+  const olb::CePlan c = olb::ce_plan(M, N);
+  const int cols = c.block_n / 4, full = N / c.tile_n, rest = N - full * c.tile_n;
+  return full * ((c.tile_n + cols - 1) / cols) + (rest + cols - 1) / cols;
 }
 
 extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
@@ -1631,7 +1705,8 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
       (reinterpret_cast<uintptr_t>(d->B) & 15) || (reinterpret_cast<uintptr_t>(d->C) & 15))
     return -10;
   const int epi = d->epilogue;
-  int block_n = d->block_n, ce_pair = 0;
+  int block_n = d->block_n;
+  CePlan plan{0, 0, 0};
   if (epi == OLB_EPI_SWIGLU) {
     // N = width of act; B / B2 = gate / up weights (K-major, same layout); C = gate | up [rows, 2 N]; C2 = act [rows, N]
     if (d->N % 128 || d->B2 == nullptr || d->C2 == nullptr || d->b_mn_major || d->a_mn_major || d->accumulate ||
@@ -1655,7 +1730,8 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
         (d->ce_repair && (d->ce_flags == nullptr || d->ce_max == nullptr)) || (d->ce_flags != nullptr && d->ce_max == nullptr) ||
         (d->ce_part != nullptr && d->ce_part_ld < d->M) || (d->ce_overlap && d->ce_repair))
       return -18;
-    block_n = olb_gemm_ce_block_n(d->M, d->N, &ce_pair);
+    plan = ce_plan(d->M, d->N);
+    block_n = plan.block_n;
   } else if (epi == OLB_EPI_ROWSCALE) {
     if (d->row_scale == nullptr || d->accumulate || d->out_fp32 || d->mode != OLB_GEMM_DENSE || d->n_peers || d->k_splits > 1 ||
         block_n != 0)
@@ -1677,7 +1753,7 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   // (ragged-M: only when the caller padded the expert groups to 256 rows; the dense all-gather / reduce-scatter
   // variants, whose peers own multiples of 128 rows, stay on the single-CTA kernel)
   const bool pair_shape = d->block_n == 0 && block_n == 256 && d->blk_range == nullptr && d->M >= 256 && num_sms >= 2 &&
-                          (epi == OLB_EPI_SWIGLU || epi == OLB_EPI_SWIGLU_BWD || (epi == OLB_EPI_CE && ce_pair) ||
+                          (epi == OLB_EPI_SWIGLU || epi == OLB_EPI_SWIGLU_BWD || (epi == OLB_EPI_CE && plan.pair) ||
                            (epi != OLB_EPI_CE && (d->N % 256 == 0 || d->N >= 2048 ||
                                                   (d->wide_tiles && (256 - d->N % 256) * 8 <= d->N))));
   const bool use_pair = pair_kernel_enabled() && pair_shape &&
@@ -1696,13 +1772,18 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   TensorMaps tm;
   int rc;
   // A: K-major -> global [a_rows, K] (inner K); MN-major -> global [K rows, M] (inner M).
+  // The cross-entropy product of a few rows loads only these (in eights) of the 128 rows of A that the tensor core reads;
+  // what the others hold reaches no row that is used.  (Rows beyond the tensor cost more than rows inside it: 200 us for
+  // one row against 128256 x 4096, 161 us for 64.)
+  const int a_box_rows = epi == OLB_EPI_CE && d->M < BLOCK_M ? (d->M + 7) / 8 * 8 : BLOCK_M;
   if (!d->a_mn_major)
-    rc = make_tmap_2d_bf16(&tm.a, d->A, d->K, d->a_rows, d->lda * 2, BLOCK_K, BLOCK_M);
+    rc = make_tmap_2d_bf16(&tm.a, d->A, d->K, d->a_rows, d->lda * 2, BLOCK_K, a_box_rows);
   else
     rc = make_tmap_2d_bf16(&tm.a, d->A, d->M, d->a_rows, d->lda * 2, 64, BLOCK_K);
   if (rc) return rc;
   int kb_split = 0;
-  const int b_box_rows = use_pair ? 128 : block_n;   // a CTA of a pair stages half of the tile's B rows
+  // a CTA of a pair stages half of the tile's B rows
+  const int b_box_rows = use_pair ? 128 : (epi == OLB_EPI_CE ? plan.tile_n : block_n);
   if (epi == OLB_EPI_SWIGLU) {
     rc = make_tmap_2d_bf16(&tm.b, d->B, d->K, d->b_rows, d->ldb * 2, BLOCK_K, 128);
     if (!rc) rc = make_tmap_2d_bf16(&tm.b2, d->B2, d->K, d->b_rows, d->ldb * 2, BLOCK_K, 128);
@@ -1767,7 +1848,9 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   p.ce_flags = d->ce_flags;
   p.ce_repair = d->ce_repair;
   p.ce_overlap = d->ce_overlap;
-  p.ce_grow = static_cast<float>(1.0 + 1.4e-8 / 16 * d->K);
+  p.ce_tile_n = plan.tile_n;
+  p.ce_a_rows = a_box_rows;
+  p.ce_grow = static_cast<float>(1.4426950408889634 * (1.0 + 1.4e-8 / 16 * d->K));
   p.ce_store = epi == OLB_EPI_CE && d->C != nullptr;
   p.c_part_rows = d->mode == OLB_GEMM_RAGGED_K ? d->M : 0;
   p.k_splits = 1;
@@ -1804,11 +1887,7 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
     if (rc) return rc;
     p.c_tma = 1;
   } else if (epi == OLB_EPI_CE) {
-    if (p.ce_store) {
-      rc = make_tmap_2d(&tm.c, d->C, d->N, d->M, d->ldc * 2, 64, 32, false);
-      if (rc) return rc;
-      p.c_tma = 1;
-    }
+    if (p.ce_store && d->ldc < (d->N + 63) / 64 * 64) return -18;  // whole chunks of 64 columns are written
   } else if (!d->accumulate) {
     const uint64_t esz = d->out_fp32 ? 4 : 2;
     uint64_t rows = p.k_splits > 1 ? static_cast<uint64_t>(p.c_part_rows) * p.k_splits : d->M;

@@ -32,7 +32,7 @@ __device__ __forceinline__ void lce_count(const long long* __restrict__ targets,
                                           float* __restrict__ inv_count) {
   __shared__ int s[LCE_WARPS];
   int c = 0;  // n < 2^31
-#pragma unroll 4
+#pragma unroll 16
   for (long long i = threadIdx.x; i < n; i += LCE_THREADS) {
     const long long t = targets[i];
     c += (t >= 0 && t < V) ? 1 : 0;
@@ -198,6 +198,7 @@ lce_finish_kernel(const olb_lce_finish_desc d) {
   if (!s_last) return;
   __threadfence();
   float acc = 0.f;
+#pragma unroll 16
   for (long long i = threadIdx.x; i < d.n_all; i += LCE_THREADS) acc += __ldcg(d.loss_all + i);
   acc = warp_sum(acc);
   if (lane == 0) s_factor[warp] = acc;
@@ -236,6 +237,7 @@ lce_scale_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, const 
 }
 
 // 8 columns per thread; the parts are summed in their order.
+template <bool ACCUMULATE>
 __global__ void __launch_bounds__(LCE_THREADS)
 lce_sum_parts_kernel(const float* __restrict__ part, int nparts, long long part_rows, int rows, int H,
                      const float* __restrict__ row_factor, __nv_bfloat16* __restrict__ out) {
@@ -253,7 +255,13 @@ lce_sum_parts_kernel(const float* __restrict__ part, int nparts, long long part_
       a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
       b.x += v.x; b.y += v.y; b.z += v.z; b.w += v.w;
     }
-    const float f = row_factor[row];
+    const float f = row_factor ? row_factor[row] : 1.f;
+    if (ACCUMULATE) {  // (only without row factors)
+      const uint4 o = reinterpret_cast<const uint4*>(out)[i];
+      const float2 p = unpack_bf16(o.x), q = unpack_bf16(o.y), r = unpack_bf16(o.z), t = unpack_bf16(o.w);
+      a.x += p.x; a.y += p.y; a.z += q.x; a.w += q.y;
+      b.x += r.x; b.y += r.y; b.z += t.x; b.w += t.y;
+    }
     reinterpret_cast<uint4*>(out)[i] = make_uint4(pack_bf16(f * a.x, f * a.y), pack_bf16(f * a.z, f * a.w),
                                                   pack_bf16(f * b.x, f * b.y), pack_bf16(f * b.z, f * b.w));
   }
@@ -300,7 +308,7 @@ extern "C" int olb_lce_prep(const void* x, long long ldx, const void* w, long lo
   const auto* xb = static_cast<const __nv_bfloat16*>(x);
   const auto* wb = static_cast<const __nv_bfloat16*>(w);
   const int extra = count != nullptr ? 1 : 0;
-  if (rows <= 148)
+  if (rows <= 148 * 8)
     lce_prep_kernel<true><<<rows + extra, LCE_THREADS, 0, stream>>>(xb, ldx, wb, ldw, targets, rows, H, V, ref, ce_max,
                                                                     ce_flags, ticket, all_targets, n_all, count);
   else
@@ -334,12 +342,13 @@ extern "C" int olb_lce_scale_rows(const void* x, long long ldx, const float* fac
 }
 
 extern "C" int olb_lce_sum_parts(const float* part, int nparts, long long part_rows, int rows, int H, const float* row_factor,
-                                 void* out, cudaStream_t stream) {
-  if (H % 8 || misaligned(part) || misaligned(out) || nparts < 1) return -1;
+                                 void* out, int accumulate, cudaStream_t stream) {
+  if (H % 8 || misaligned(part) || misaligned(out) || nparts < 1 || (accumulate && row_factor)) return -1;
   if (rows <= 0) return 0;
   const long long blocks = (static_cast<long long>(rows) * (H / 8) + LCE_THREADS - 1) / LCE_THREADS;
-  lce_sum_parts_kernel<<<static_cast<int>(blocks < 148 * 16 ? blocks : 148 * 16), LCE_THREADS, 0, stream>>>(
-      part, nparts, part_rows, rows, H, row_factor, static_cast<__nv_bfloat16*>(out));
+  const int grid = static_cast<int>(blocks < 148 * 16 ? blocks : 148 * 16);
+  auto* kernel = accumulate ? lce_sum_parts_kernel<true> : lce_sum_parts_kernel<false>;
+  kernel<<<grid, LCE_THREADS, 0, stream>>>(part, nparts, part_rows, rows, H, row_factor, static_cast<__nv_bfloat16*>(out));
   return launched();
 }
 

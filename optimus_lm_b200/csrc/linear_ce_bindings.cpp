@@ -148,7 +148,7 @@ void input_gradient(const Problem& p, int64_t r0, int64_t rows, const void* E, c
   d.c_part_rows = static_cast<int>(part_rows);
   check(olb_gemm_bf16(&d, p.stream), "olb_gemm_bf16 (input gradient)");
   check(olb_lce_sum_parts(partial.data_ptr<float>(), parts, part_rows, static_cast<int>(rows), static_cast<int>(p.H),
-                          row_factor, row_ptr(dx, r0), p.stream),
+                          row_factor, row_ptr(dx, r0), 0, p.stream),
         "olb_lce_sum_parts");
 }
 
@@ -170,6 +170,21 @@ void weight_gradient(const Problem& p, int64_t rows, const void* E, const void* 
   d.wide_tiles = 1;
   d.status = p.status;
   d.out_fp32 = dw.scalar_type() == at::kFloat;
+  const int parts = d.out_fp32 ? 1 : split_parts(p.V, p.H, rows);
+  if (parts > 1) {  // a small weight and a long batch
+    const int64_t part_rows = round_up(p.V, 128);
+    at::Tensor partial = at::empty({parts * part_rows, p.H}, p.x.options().dtype(at::kFloat));
+    d.C = partial.data_ptr();
+    d.ldc = p.H;
+    d.out_fp32 = 1;
+    d.k_splits = parts;
+    d.c_part_rows = static_cast<int>(part_rows);
+    check(olb_gemm_bf16(&d, p.stream), "olb_gemm_bf16 (weight gradient)");
+    check(olb_lce_sum_parts(partial.data_ptr<float>(), parts, part_rows, static_cast<int>(p.V), static_cast<int>(p.H), nullptr,
+                            dw.data_ptr(), add, p.stream),
+          "olb_lce_sum_parts");
+    return;
+  }
   if (d.out_fp32)
     d.c_reduce = add;
   else
@@ -201,11 +216,14 @@ at::Tensor linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Ten
     kept = {PIECE, at::empty({0, p.lde}, x.options()), at::empty({0}, f32)};
     return out;
   }
-  int64_t rows_max = piece_rows(p.T, grad ? 2 * p.lde : 4 * ((p.V + 63) / 64), max_bytes);
+  int64_t rows_max = piece_rows(p.T, grad ? 2 * p.lde : 4 * ((p.V + 15) / 16), max_bytes);
   const bool single = rows_max >= p.T;
   const bool store = grad && (single || reduction != NONE);   // several pieces of losses per row: exponentials again later
-  if (grad && !single && reduction == NONE) rows_max = piece_rows(p.T, 4 * ((p.V + 63) / 64), max_bytes);
-  const int64_t ntiles_most = (p.V + 63) / 64;
+  if (grad && !single && reduction == NONE) rows_max = piece_rows(p.T, 4 * ((p.V + 15) / 16), max_bytes);
+  // sums per row, of whole pieces and of a shorter last one
+  const int64_t last = p.T - (p.T - 1) / rows_max * rows_max;
+  const int64_t ntiles_most = std::max(olb_gemm_ce_slices(static_cast<int>(std::min(rows_max, p.T)), static_cast<int>(p.V)),
+                                       olb_gemm_ce_slices(static_cast<int>(last), static_cast<int>(p.V)));
 
   at::Tensor loss_rows = at::empty({p.T}, f32);
   at::Tensor out = reduction == NONE ? loss_rows : at::empty({}, f32);
@@ -236,7 +254,6 @@ at::Tensor linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Ten
   }
   for (int64_t r0 = 0; r0 < p.T; r0 += rows_max) {
     const int64_t rows = std::min(rows_max, p.T - r0);
-    const int bn = olb_gemm_ce_block_n(static_cast<int>(rows), static_cast<int>(p.V), nullptr);
     check(olb_lce_prep(row_ptr(x, r0), x.stride(0), w.data_ptr(), w.stride(0), ptr_i64(p.targets, r0), static_cast<int>(rows),
                        static_cast<int>(p.H), static_cast<int>(p.V), ref, top, flags, ticket, ptr_i64(p.targets, 0), p.T,
                        reduction == MEAN && r0 == 0 ? count : nullptr, p.stream),
@@ -245,7 +262,7 @@ at::Tensor linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Ten
     olb_lce_finish_desc f{};
     f.part = part.data_ptr<float>();
     f.part_ld = rows_max;
-    f.ntiles = static_cast<int>((p.V + bn - 1) / bn);
+    f.ntiles = olb_gemm_ce_slices(static_cast<int>(rows), static_cast<int>(p.V));
     f.ref = ref;
     f.ce_max = top;
     f.targets = ptr_i64(p.targets, r0);

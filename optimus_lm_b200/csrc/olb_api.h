@@ -100,9 +100,9 @@ typedef struct {
   const float* row_scale;    // epilogue == OLB_EPI_ROWSCALE (DENSE, bf16 C): row r of the product times row_scale[r]
   // Cross-entropy product (epilogue == OLB_EPI_CE; DENSE, K-major operands): A = hidden states, B = the head's weight
   // [N, K] with any number of rows N.  Row r has its target in ce_targets[r] (outside [0, N): no target) and a reference
-  // ce_ref[r]; with l the logits, C (may be NULL) receives exp(l - ref) as bf16, zeros for rows without a target, and
-  // ce_part[tile * ce_part_ld + r] (may be NULL) the sum of exp(l - ref) over column tile `tile` (olb_gemm_ce_block_n
-  // columns each) without the target's column.  ce_flags (may be NULL; 1 + ceil(M / 128) ints and ce_max M words, all
+  // ce_ref[r]; with l the logits, C (may be NULL) receives exp(l - ref) as bf16, zeros for rows without a target and up to
+  // the next multiple of 32 columns, and ce_part[i * ce_part_ld + r] (may be NULL) the sum of exp(l - ref) over the i-th
+  // of olb_gemm_ce_slices(M, N) slices of the columns without the target's column.  ce_flags (may be NULL; 1 + ceil(M / 128) ints and ce_max M words, all
   // zero): a row whose largest logit exceeds its reference by more than 40 has it recorded in ce_max and its block of
   // 128 rows flagged.  ce_repair: the same product for the flagged blocks alone, rows with a recorded maximum against that.
   const long long* ce_targets;
@@ -118,8 +118,8 @@ typedef struct {
 } olb_gemm_desc;
 
 int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream);
-// Columns of a statistics tile of the cross-entropy product; *pair (may be NULL): CTA pairs take 256 x 256 tiles.
-int olb_gemm_ce_block_n(int M, int N, int* pair);
+// Slices of N for which the cross-entropy product of M rows writes a sum of its own (at most ceil(N / 16) + 3).
+int olb_gemm_ce_slices(int M, int N);
 
 // ---------------------------------------------------------------- normalisation (norm.cu)
 // y = x * rsqrt(mean(x^2) + eps) * w   (w may be NULL).  rstd [rows] fp32 is saved for backward.
@@ -277,9 +277,10 @@ int olb_lce_patch(const float* prob, const long long* targets, int rows, int V, 
 // row_factor[r] = factor[r] * grad[r * grad_stride] and, when xs is not NULL, xs[r, :] = bf16(row_factor[r] * x[r, :]).
 int olb_lce_scale_rows(const void* x, long long ldx, const float* factor, const float* grad, long long grad_stride, int rows,
                        int H, float* row_factor, void* xs, cudaStream_t stream);
-// out[r, :] = bf16(row_factor[r] * sum_s part[s * part_rows + r, :]) in the order of s.
+// out[r, :] = bf16(row_factor[r] * sum_s part[s * part_rows + r, :]) in the order of s (row_factor NULL: 1, and then with
+// accumulate out[r, :] is added before the rounding).
 int olb_lce_sum_parts(const float* part, int nparts, long long part_rows, int rows, int H, const float* row_factor, void* out,
-                      cudaStream_t stream);
+                      int accumulate, cudaStream_t stream);
 // dst (bf16) = (accumulate ? dst : 0) + *grad * src (NULL: 1), src fp32 or (src_bf16) bf16, n elements.
 int olb_lce_scale_out(const void* src, int src_bf16, long long n, const float* grad, void* dst, int accumulate,
                       cudaStream_t stream);

@@ -106,7 +106,9 @@ def check(x, w, t, reduction, twice=False, **kw):
 
 SIZES = [(1, 8, 1), (1, 64, 40), (2, 8, 2), (3, 72, 100), (31, 16, 63), (64, 512, 1000), (127, 128, 256), (128, 64, 257),
          (129, 200, 255), (130, 1000, 3001), (256, 256, 512), (257, 40, 65), (300, 264, 777), (513, 512, 1024),
-         (700, 2048, 5000), (1100, 136, 300)]
+         (700, 2048, 5000), (1100, 136, 300),
+         # few rows: tiles of 224, 192, 160 and 96 columns
+         (3, 16, 128256), (5, 64, 50304), (9, 24, 70001), (70, 40, 14001), (150, 16, 40000)]
 
 
 @pytest.mark.parametrize("T,H,V", SIZES)
