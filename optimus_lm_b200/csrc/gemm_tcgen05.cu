@@ -85,6 +85,7 @@ struct GemmParams {
   // [s * c_part_rows, + M) of C.  (Ragged-K: part = expert, c_part_rows = M.)
   int k_splits, split_kb;
   int c_part_rows;
+  int overlap;                 // the launch before this one may still be running: the epilogue waits for it
   int c_reduce;                // fp32 output added to C by the stores themselves (bulk reduction), no read in the kernel
   const float* row_scale;      // EPI_ROWSCALE: row r of the product is multiplied by row_scale[r] before it is rounded
   // EPI_CE: see epilogue_ce.
@@ -97,7 +98,6 @@ struct GemmParams {
   float ce_grow;               // see epilogue_ce
   int ce_a_rows;               // rows of A in a tile's boxes: 128, or fewer in a launch of one row block
   int ce_tile_n;               // columns per tile, a multiple of 32 up to BLOCK_N
-  int ce_overlap;              // the launch before this one may still be running: wait for it before its results are read
   int ce_repair;               // only the flagged row blocks, with their rows' recorded maxima as references
   int ce_store;                // the exponentials are written to C
 };
@@ -855,8 +855,12 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
   constexpr uint32_t TMEM_COLS = (2 * BLOCK_N < 32) ? 32 : 2 * BLOCK_N;
   static_assert(EPI != EPI_SWIGLU || BLOCK_N == 256, "the SwiGLU epilogue pairs 128 gate with 128 up columns");
 
+  if (p.overlap) grid_launch_dependents();
   if constexpr (EPI == EPI_CE) {
-    if (p.ce_repair && p.ce_flags[0] == 0) return;  // nothing to repair: the same answer in every CTA
+    if (p.ce_repair) {
+      if (p.overlap) grid_dependency_wait();  // every thread: this launch ends after the one before it
+      if (p.ce_flags[0] == 0) return;         // nothing to repair: the same answer in every CTA
+    }
   }
 
   extern __shared__ uint8_t smem_raw[];
@@ -1046,9 +1050,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
     }
   } else if (warp < 2 + epilogue_warps(EPI)) {
     // ------------------------------------------------------------ epilogue (warps 2..5)
-    if constexpr (EPI == EPI_CE) {
-      if (p.ce_overlap) grid_dependency_wait();
-    }
+    if (p.overlap) grid_dependency_wait();
     const int lane_group = warp & 3;  // TMEM lanes [32*lane_group, +32) belong to this warp
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -1178,8 +1180,12 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
   constexpr int BLOCK_N = 256;
   constexpr uint32_t TMEM_COLS = 512;
 
+  if (p.overlap) grid_launch_dependents();
   if constexpr (EPI == EPI_CE) {
-    if (p.ce_repair && p.ce_flags[0] == 0) return;  // nothing to repair: the same answer in every CTA
+    if (p.ce_repair) {
+      if (p.overlap) grid_dependency_wait();  // every thread: this launch ends after the one before it
+      if (p.ce_flags[0] == 0) return;         // nothing to repair: the same answer in every CTA
+    }
   }
 
   extern __shared__ uint8_t smem_raw[];
@@ -1364,9 +1370,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
     }
   } else if (warp < 2 + epilogue_warps(EPI)) {
     // ------------------------------------------------------------ epilogue (warps 2..5 of both CTAs, own 128 rows)
-    if constexpr (EPI == EPI_CE) {
-      if (p.ce_overlap) grid_dependency_wait();
-    }
+    if (p.overlap) grid_dependency_wait();
     const int lane_group = warp & 3;
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -1573,8 +1577,8 @@ static int launch(const TensorMaps& tm, const PeerArg<PEER>& peers, const GemmPa
   const long long tiles = nm * nn * (p.mode == OLB_GEMM_RAGGED_K ? p.num_experts : (p.k_splits > 1 ? p.k_splits : 1));
   int grid = static_cast<int>(tiles < num_sms ? tiles : num_sms);
   if (grid <= 0) return 0;
-  if constexpr (EPI == EPI_CE) {
-    if (p.ce_overlap)
+  if constexpr (!PEER && (EPI == EPI_CE || EPI == EPI_PLAIN || EPI == EPI_ROWSCALE)) {
+    if (p.overlap)
       return launch_overlapped(gemm_bf16_kernel<BLOCK_N, PEER, EPI>, grid, num_threads(PEER, EPI), L::TOTAL, stream, tm, peers, p);
   }
   gemm_bf16_kernel<BLOCK_N, PEER, EPI><<<grid, num_threads(PEER, EPI), L::TOTAL, stream>>>(
@@ -1602,8 +1606,8 @@ static int launch_pair(const TensorMaps& tm, const PeerArg<PEER>& peers, const G
   const int max_pairs = num_sms / 2;
   const int pairs = static_cast<int>(tiles < max_pairs ? tiles : max_pairs);
   if (pairs <= 0) return 0;
-  if constexpr (EPI == EPI_CE) {
-    if (p.ce_overlap)
+  if constexpr (!PEER && (EPI == EPI_CE || EPI == EPI_PLAIN || EPI == EPI_ROWSCALE)) {
+    if (p.overlap)
       return launch_overlapped(gemm_bf16_pair_kernel<PEER, EPI>, 2 * pairs, num_threads(PEER, EPI), L::TOTAL, stream, tm, peers, p);
   }
   gemm_bf16_pair_kernel<PEER, EPI><<<2 * pairs, num_threads(PEER, EPI), L::TOTAL, stream>>>(
@@ -1701,6 +1705,7 @@ extern "C" int olb_gemm_ce_slices(int M, int N) {
 extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   using namespace olb;
   if (d->M <= 0 || d->N <= 0) return 0;
+  if (d->overlap && (d->mode != OLB_GEMM_DENSE || d->n_peers || d->accumulate || d->c_reduce)) return -23;
   if ((d->lda % 8) || (d->ldb % 8) || (d->ldc % 8) || (d->N % 8 && d->epilogue != OLB_EPI_CE) || (reinterpret_cast<uintptr_t>(d->A) & 15) ||
       (reinterpret_cast<uintptr_t>(d->B) & 15) || (reinterpret_cast<uintptr_t>(d->C) & 15))
     return -10;
@@ -1728,7 +1733,7 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
     if (d->a_mn_major || d->b_mn_major || d->accumulate || d->out_fp32 || d->mode != OLB_GEMM_DENSE || d->n_peers ||
         d->k_split || d->k_splits > 1 || d->ce_targets == nullptr || d->ce_ref == nullptr ||
         (d->ce_repair && (d->ce_flags == nullptr || d->ce_max == nullptr)) || (d->ce_flags != nullptr && d->ce_max == nullptr) ||
-        (d->ce_part != nullptr && d->ce_part_ld < d->M) || (d->ce_overlap && d->ce_repair))
+        (d->ce_part != nullptr && d->ce_part_ld < d->M))
       return -18;
     plan = ce_plan(d->M, d->N);
     block_n = plan.block_n;
@@ -1847,7 +1852,7 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   p.ce_part_ld = d->ce_part_ld;
   p.ce_flags = d->ce_flags;
   p.ce_repair = d->ce_repair;
-  p.ce_overlap = d->ce_overlap;
+  p.overlap = d->overlap;
   p.ce_tile_n = plan.tile_n;
   p.ce_a_rows = a_box_rows;
   p.ce_grow = static_cast<float>(1.4426950408889634 * (1.0 + 1.4e-8 / 16 * d->K));

@@ -57,7 +57,7 @@ lce_prep_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, const __nv_b
                 unsigned* __restrict__ ce_max, int* __restrict__ ce_flags, unsigned* __restrict__ ticket,
                 const long long* __restrict__ all_targets, long long n_all, float* __restrict__ count) {
   // the product may start: nothing of it but its epilogue needs what this kernel writes
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  grid_launch_dependents();
   if (count != nullptr && blockIdx.x == gridDim.x - 1) {
     lce_count(all_targets, n_all, V, count, count + 1);
     return;
@@ -137,6 +137,7 @@ lce_finish_kernel(const olb_lce_finish_desc d) {
   __shared__ float s_sum[TILES][LCE_ROWS];
   __shared__ float s_factor[LCE_ROWS];
   __shared__ bool s_last;
+  grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row0 = blockIdx.x * LCE_ROWS;
   const int sub = threadIdx.x % LCE_ROWS, row = row0 + sub;
@@ -227,6 +228,7 @@ __global__ void __launch_bounds__(LCE_THREADS)
 lce_scale_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, const float* __restrict__ factor,
                       const float* __restrict__ grad, long long grad_stride, int rows, int H, float* __restrict__ row_factor,
                       __nv_bfloat16* __restrict__ xs) {
+  grid_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int row = blockIdx.x * LCE_WARPS + (threadIdx.x >> 5);
   if (row >= rows) return;
@@ -241,6 +243,7 @@ template <bool ACCUMULATE>
 __global__ void __launch_bounds__(LCE_THREADS)
 lce_sum_parts_kernel(const float* __restrict__ part, int nparts, long long part_rows, int rows, int H,
                      const float* __restrict__ row_factor, __nv_bfloat16* __restrict__ out) {
+  grid_dependency_wait();
   const int vecs = H / 8;
   const long long total = static_cast<long long>(rows) * vecs;
   for (long long i = blockIdx.x * static_cast<long long>(LCE_THREADS) + threadIdx.x; i < total;
@@ -294,6 +297,20 @@ lce_scale_out_kernel(const void* __restrict__ src_, long long vecs, const float*
 }
 
 static bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+// A launch that may begin before the one before it on the stream has ended: the kernel waits for that itself.
+template <typename... P, typename... A>
+static int launch_waiting(void (*kernel)(P...), int grid, cudaStream_t stream, A... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(LCE_THREADS);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...) == cudaSuccess ? 0 : -2;
+}
 static int launched() { return cudaGetLastError() == cudaSuccess ? 0 : -2; }
 
 }  // namespace olb
@@ -320,8 +337,7 @@ extern "C" int olb_lce_prep(const void* x, long long ldx, const void* w, long lo
 extern "C" int olb_lce_finish(const olb_lce_finish_desc* d, cudaStream_t stream) {
   if ((d->xs && (d->H % 8 || d->ldx % 8 || misaligned(d->x) || misaligned(d->xs))) || (d->total && !d->ticket)) return -1;
   if (d->rows <= 0) return 0;
-  lce_finish_kernel<<<(d->rows + LCE_ROWS - 1) / LCE_ROWS, LCE_THREADS, 0, stream>>>(*d);
-  return launched();
+  return launch_waiting(lce_finish_kernel, (d->rows + LCE_ROWS - 1) / LCE_ROWS, stream, *d);
 }
 
 extern "C" int olb_lce_patch(const float* prob, const long long* targets, int rows, int V, void* E, long long lde,
@@ -348,8 +364,7 @@ extern "C" int olb_lce_sum_parts(const float* part, int nparts, long long part_r
   const long long blocks = (static_cast<long long>(rows) * (H / 8) + LCE_THREADS - 1) / LCE_THREADS;
   const int grid = static_cast<int>(blocks < 148 * 16 ? blocks : 148 * 16);
   auto* kernel = accumulate ? lce_sum_parts_kernel<true> : lce_sum_parts_kernel<false>;
-  kernel<<<grid, LCE_THREADS, 0, stream>>>(part, nparts, part_rows, rows, H, row_factor, static_cast<__nv_bfloat16*>(out));
-  return launched();
+  return launch_waiting(kernel, grid, stream, part, nparts, part_rows, rows, H, row_factor, static_cast<__nv_bfloat16*>(out));
 }
 
 extern "C" int olb_lce_scale_out(const void* src, int src_bf16, long long n, const float* grad, void* dst, int accumulate,

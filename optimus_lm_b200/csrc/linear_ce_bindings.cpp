@@ -107,17 +107,18 @@ void product(const Problem& p, int64_t r0, int64_t rows, const float* ref, unsig
   d.ce_flags = flags;
   d.ce_part = part;
   d.ce_part_ld = part_ld;
-  d.ce_overlap = behind_prep;
+  d.overlap = behind_prep;
   check(olb_gemm_bf16(&d, p.stream), "olb_gemm_bf16 (cross entropy)");
   if (flags) {
-    d.ce_overlap = 0;
+    d.overlap = 1;
     d.ce_repair = 1;
     check(olb_gemm_bf16(&d, p.stream), "olb_gemm_bf16 (cross entropy, repair)");
   }
 }
 
-// dx[r0 .. r0 + rows) = row_factor * (E W)
-void input_gradient(const Problem& p, int64_t r0, int64_t rows, const void* E, const float* row_factor, at::Tensor& dx) {
+// dx[r0 .. r0 + rows) = row_factor * (E W).  behind_factors: the launch before it makes row_factor and not E.
+void input_gradient(const Problem& p, int64_t r0, int64_t rows, const void* E, const float* row_factor, at::Tensor& dx,
+                    bool behind_factors) {
   const int parts = split_parts(rows, p.H, p.V);
   olb_gemm_desc d{};
   d.A = E;
@@ -131,6 +132,7 @@ void input_gradient(const Problem& p, int64_t r0, int64_t rows, const void* E, c
   d.K = static_cast<int>(p.V);
   d.b_mn_major = 1;
   d.wide_tiles = 1;
+  d.overlap = behind_factors;
   d.status = p.status;
   d.ldc = p.H;
   if (parts == 1) {
@@ -225,11 +227,12 @@ at::Tensor linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Ten
   const int64_t ntiles_most = std::max(olb_gemm_ce_slices(static_cast<int>(std::min(rows_max, p.T)), static_cast<int>(p.V)),
                                        olb_gemm_ce_slices(static_cast<int>(last), static_cast<int>(p.V)));
 
-  at::Tensor loss_rows = at::empty({p.T}, f32);
-  at::Tensor out = reduction == NONE ? loss_rows : at::empty({}, f32);
-  // small per-row and per-launch words: ref, top, flags, ticket, count, 1 / count
-  at::Tensor words = at::empty({2 * rows_max + (rows_max + 127) / 128 + 1 + 3}, f32);
-  float* ref = words.data_ptr<float>();
+  at::Tensor out = reduction == NONE ? at::empty({p.T}, f32) : at::empty({}, f32);
+  // small per-row and per-launch words: (losses,) ref, top, flags, ticket, count, 1 / count
+  const int64_t losses = reduction == NONE ? 0 : p.T;
+  at::Tensor words = at::empty({losses + 2 * rows_max + (rows_max + 127) / 128 + 1 + 3}, f32);
+  float* loss_rows = reduction == NONE ? out.data_ptr<float>() : words.data_ptr<float>();
+  float* ref = words.data_ptr<float>() + losses;
   unsigned* top = reinterpret_cast<unsigned*>(ref + rows_max);
   int* flags = reinterpret_cast<int*>(top + rows_max);
   unsigned* ticket = reinterpret_cast<unsigned*>(flags + (rows_max + 127) / 128 + 1);
@@ -269,7 +272,7 @@ at::Tensor linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Ten
     f.rows = static_cast<int>(rows);
     f.V = static_cast<int>(p.V);
     f.H = static_cast<int>(p.H);
-    f.loss = loss_rows.data_ptr<float>() + r0;
+    f.loss = loss_rows + r0;
     if (prob.defined()) {
       f.prob = prob.data_ptr<float>() + r0;
       f.lse = lse.data_ptr<float>() + r0;
@@ -287,14 +290,14 @@ at::Tensor linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Ten
     }
     if (reduction != NONE && r0 + rows == p.T) {
       f.ticket = ticket;
-      f.loss_all = loss_rows.data_ptr<float>();
+      f.loss_all = loss_rows;
       f.n_all = p.T;
       f.total = out.data_ptr<float>();
       f.total_scale = reduction == MEAN ? count : nullptr;
     }
     check(olb_lce_finish(&f, p.stream), "olb_lce_finish");
     if (in_forward) {
-      if (need_dx) input_gradient(p, r0, rows, E.data_ptr(), factor.data_ptr<float>(), dx);
+      if (need_dx) input_gradient(p, r0, rows, E.data_ptr(), factor.data_ptr<float>(), dx, false);
       if (need_dw) weight_gradient(p, rows, E.data_ptr(), xs.data_ptr(), dw32, r0 > 0);
     }
   }
@@ -327,7 +330,7 @@ std::vector<at::Tensor> linear_ce_bwd(const at::Tensor& x, const at::Tensor& w, 
                            grad.dim() == 0 ? 0 : 1, static_cast<int>(p.T), static_cast<int>(p.H), row_factor.data_ptr<float>(),
                            need_dw ? xs.data_ptr() : nullptr, p.stream),
         "olb_lce_scale_rows");
-  if (need_dx) input_gradient(p, 0, p.T, E.data_ptr(), row_factor.data_ptr<float>(), dx);
+  if (need_dx) input_gradient(p, 0, p.T, E.data_ptr(), row_factor.data_ptr<float>(), dx, true);
   if (need_dw) weight_gradient(p, p.T, E.data_ptr(), xs.data_ptr(), dw, accumulate);
   return {dx, dw};
 }
@@ -382,7 +385,7 @@ std::vector<at::Tensor> linear_ce_bwd_again(const at::Tensor& x, const at::Tenso
                              static_cast<int>(rows), static_cast<int>(p.H), row_factor.data_ptr<float>(),
                              need_dw ? xs.data_ptr() : nullptr, p.stream),
           "olb_lce_scale_rows");
-    if (need_dx) input_gradient(p, r0, rows, E.data_ptr(), row_factor.data_ptr<float>(), dx);
+    if (need_dx) input_gradient(p, r0, rows, E.data_ptr(), row_factor.data_ptr<float>(), dx, false);
     if (need_dw) weight_gradient(p, rows, E.data_ptr(), xs.data_ptr(), dw32, r0 > 0);
   }
   if (need_dw)
@@ -395,6 +398,10 @@ struct GradHolder : torch::CustomClassHolder {
   pybind11::object obj;
   explicit GradHolder(pybind11::object o) : obj(std::move(o)) {}
   ~GradHolder() override {
+    if (!Py_IsInitialized()) {  // a graph that outlives the interpreter
+      obj.release();
+      return;
+    }
     pybind11::gil_scoped_acquire gil;
     obj = pybind11::object();
   }
@@ -408,7 +415,8 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
                             const at::Tensor& status, const c10::intrusive_ptr<GradHolder>& holder) {
     Kept kept;
     at::Tensor out = linear_ce_fwd(x, w, targets, reduction, need_dx, need_dw, max_bytes, status, kept);
-    ctx->save_for_backward({x, w, targets, status, kept.a, kept.b});
+    ctx->save_for_backward({x, w, targets, kept.a, kept.b});
+    ctx->saved_data["status"] = status;  // cleared in place by whoever reads it
     ctx->saved_data["kind"] = kept.kind;
     ctx->saved_data["need"] = static_cast<int64_t>(need_dx) + 2 * static_cast<int64_t>(need_dw);
     ctx->saved_data["max_bytes"] = max_bytes;
@@ -430,7 +438,8 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
       into = holder->obj.attr("buf").cast<at::Tensor>();
       add = holder->obj.attr("ready").cast<bool>();
     }
-    const at::Tensor &x = saved[0], &w = saved[1], &targets = saved[2], &status = saved[3], &a = saved[4], &b = saved[5];
+    const at::Tensor &x = saved[0], &w = saved[1], &targets = saved[2], &a = saved[3], &b = saved[4];
+    const at::Tensor status = ctx->saved_data["status"].toTensor();
     auto got = kind == PIECE   ? linear_ce_bwd(x, w, targets, a, b, grad, need_dx, need_dw, into, add, status)
                : kind == SCALE ? linear_ce_bwd_scale(a, b, grad, into, add)
                                : linear_ce_bwd_again(x, w, targets, a, b, grad, need_dx, need_dw,

@@ -112,7 +112,10 @@ typedef struct {
   long long ce_part_ld;
   int* ce_flags;
   int ce_repair;
-  int ce_overlap;            // the launch before this one on the stream is olb_lce_prep: start under it
+  // DENSE, C written and not read: start while the launch before this one on the stream is still running, if that allows
+  // it; only the epilogue (row_scale, ce_*, the stores to C) waits for its end.  For a launch whose A and B do not come from
+  // the one before it.  The launch after this one may start early in turn.
+  int overlap;
   int wide_tiles;            // DENSE: CTA-pair tiles also for an N below 2048 that is no multiple of 256, where they waste
                              // at most an eighth of it
 } olb_gemm_desc;
@@ -238,8 +241,7 @@ int olb_ce_partial_bwd(const void* logits, long long ldl, const long long* label
 // The passes around the OLB_EPI_CE product; `rows` is one piece of the batch (see linear_ce.cu for the formulas).
 // ref[r] = x_r . w_t (fp32) for rows with a target t in [0, V), else 0; zeroes ce_max [rows], ce_flags
 // [1 + ceil(rows / 128)] and *ticket.  With count: count[0] = number of all_targets [n_all] in [0, V) (as fp32, rounded
-// above 2^24), count[1] = 1 / that (0 when there are none).  A product launched next (OLB_EPI_CE, ce_overlap) may
-// start before this is done.
+// above 2^24), count[1] = 1 / that (0 when there are none).  A product launched next with `overlap` starts under this.
 int olb_lce_prep(const void* x, long long ldx, const void* w, long long ldw, const long long* targets, int rows, int H,
                  int V, float* ref, unsigned* ce_max, int* ce_flags, unsigned* ticket, const long long* all_targets,
                  long long n_all, float* count, cudaStream_t stream);
@@ -269,12 +271,14 @@ typedef struct {
   const float* total_scale;
   float* total;
 } olb_lce_finish_desc;
+// (launched so that it waits for the launch before it inside the kernel)
 int olb_lce_finish(const olb_lce_finish_desc* d, cudaStream_t stream);
 // The target entries of exponentials that were taken against the log-sum-exp: E[r, t] = -prob[r] (rounded), factor[r]
 // as above with the row's gradient grad[r * grad_stride].
 int olb_lce_patch(const float* prob, const long long* targets, int rows, int V, void* E, long long lde, float* factor,
                   cudaStream_t stream);
 // row_factor[r] = factor[r] * grad[r * grad_stride] and, when xs is not NULL, xs[r, :] = bf16(row_factor[r] * x[r, :]).
+// A product launched next with `overlap` starts under this.
 int olb_lce_scale_rows(const void* x, long long ldx, const float* factor, const float* grad, long long grad_stride, int rows,
                        int H, float* row_factor, void* xs, cudaStream_t stream);
 // out[r, :] = bf16(row_factor[r] * sum_s part[s * part_rows + r, :]) in the order of s (row_factor NULL: 1, and then with

@@ -61,6 +61,8 @@ __device__ __forceinline__ bool elect_one() {
   return pred != 0;
 }
 
+// Lets the next launch on the stream start (if it was made so that it may), before this one has ended.
+__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // Until the launch before this one on the stream (programmatic dependent launch) has finished and its writes are visible.
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
