@@ -186,6 +186,7 @@ __device__ __forceinline__ unsigned clip_block_max(unsigned v, unsigned* s) {
 template <int CAP, bool INF>
 __global__ void __launch_bounds__(CLIP_THREADS, 4)
 grad_norm_kernel(const __grid_constant__ ClipTable<CAP> t, unsigned per_block, double* __restrict__ partial) {
+  grid_launch_dependents();
   __shared__ double s[CLIP_THREADS / 32];
   const unsigned begin = blockIdx.x * per_block, end = min(begin + per_block, t.pieces);
   double sum = 0.0;
@@ -236,6 +237,7 @@ template <int CAP, bool INF>
 __global__ void __launch_bounds__(CLIP_THREADS, 4)
 grad_scale_kernel(const __grid_constant__ ClipTable<CAP> t, unsigned per_block, const double* __restrict__ partial, int nparts,
                   float max_norm, float eps, float* __restrict__ norm_out) {
+  grid_dependency_wait();
   __shared__ double s[CLIP_THREADS / 32];
   const float norm = clip_norm<INF>(partial, nparts, s);
   if (blockIdx.x == 0 && threadIdx.x == 0 && norm_out) *norm_out = norm;
@@ -321,7 +323,19 @@ static int clip_run(const olb_clip_tensor* list, int n, int scale, float max_nor
     float* out = norm_out;
     while (clip_fill(t, list, n, &next, &done)) {
       const int grid = clip_grid(t.pieces, &per);
-      grad_scale_kernel<CAP, INF><<<grid, CLIP_THREADS, 0, stream>>>(t, per, partial, nparts, max_norm, eps, out);
+      // the first one is put in place under the last of the norm's launches
+      cudaLaunchAttribute attr{};
+      attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr.val.programmaticStreamSerializationAllowed = out != nullptr;
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(grid);
+      cfg.blockDim = dim3(CLIP_THREADS);
+      cfg.stream = stream;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      if (cudaLaunchKernelEx(&cfg, grad_scale_kernel<CAP, INF>, t, per, static_cast<const double*>(partial), nparts, max_norm,
+                             eps, out) != cudaSuccess)
+        return -3;
       out = nullptr;
     }
   }

@@ -48,13 +48,13 @@ c10::optional<at::Tensor> grad_clip(const pybind11::list& items, bool inf_norm, 
   c10::cuda::CUDAGuard guard(device);
   for (const at::Tensor& g : grads) {
     if (g.numel() == 0) continue;
-    at::Tensor at = g;
+    const at::Tensor* dense = &g;
     if (!g.is_non_overlapping_and_dense()) {
       TORCH_CHECK_VALUE(!scale || no_self_overlap(g), "a gradient to be scaled addresses an element more than once");
-      at = g.contiguous();
-      copies.emplace_back(g, at);
+      copies.emplace_back(g, g.contiguous());
+      dense = &copies.back().second;
     }
-    list.push_back({at.data_ptr(), at.numel(), at.scalar_type() == at::kFloat});
+    list.push_back({dense->data_ptr(), dense->numel(), dense->scalar_type() == at::kFloat});
   }
   if (scale) {
     // the same memory twice would be scaled by two blocks at once (a copy is not: whatever it shares holds the same values)

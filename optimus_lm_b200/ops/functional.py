@@ -26,15 +26,21 @@ GEMM_DENSE, GEMM_RAGGED_M, GEMM_RAGGED_K = 0, 1, 2
 
 # Device status word per GPU: kernels record bounded-wait timeouts / capacity overflow here.
 _STATUS = {}
+_STATUS_OF = {}
 
 
 def status_word(device) -> torch.Tensor:
+    t = _STATUS_OF.get(device)
+    if t is not None:
+        return t
     device = torch.device(device)
     key = (device.type, device.index if device.index is not None else torch.cuda.current_device())
     t = _STATUS.get(key)
     if t is None:
         t = torch.zeros(1, dtype=torch.int32, device=device)
         _STATUS[key] = t
+    if device.index is not None:
+        _STATUS_OF[device] = t   # found again without taking the device apart
     return t
 
 
@@ -1175,7 +1181,6 @@ def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
     return _grad_norm_reference(grads, norm_type) if grads else torch.zeros(())
 
 
-@torch.no_grad()
 def clip_grad_norm_(grads, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
     """Scale the tensors ``grads`` in place by ``min(1, max_norm / (norm + 1e-6))`` and return ``norm`` (see
     ``grad_norm``) as it was before.  The factor stays on the device: no synchronisation, and the call can be captured
@@ -1191,8 +1196,9 @@ def clip_grad_norm_(grads, max_norm: float, norm_type: float = 2.0) -> torch.Ten
         norm = extension().grad_clip(grads, norm_type == math.inf, True, max_norm, 1e-6)
         if norm is not None:
             return norm
-    norm = grad_norm(grads, norm_type)
-    factor = torch.clamp(max_norm / (norm + 1e-6), max=1.0)
-    for g in grads:
-        g.copy_(g.float() * factor if g.dtype != torch.float64 else g * factor)
+    with torch.no_grad():
+        norm = grad_norm(grads, norm_type)
+        factor = torch.clamp(max_norm / (norm + 1e-6), max=1.0)
+        for g in grads:
+            g.copy_(g.float() * factor if g.dtype != torch.float64 else g * factor)
     return norm

@@ -357,3 +357,60 @@ def test_many_rows_and_few_columns():
     x, w, t = make(5000, 64, 50, seed=31, ignored=0.1)
     check(x, w, t, "mean")
     check(x, w, t, "none", max_workspace=1 << 18)
+
+
+def test_exponentials_past_31_bits_of_elements():
+    free, _ = torch.cuda.mem_get_info()
+    if free < 40 << 30:
+        pytest.skip("needs 40 GB of free device memory")
+    T, H, V = 20000, 16, 128256   # 2.57e9 exponentials in one piece
+    x, w, t = make(T, H, V, seed=2, w_scale=0.3)
+    loss, dx, dw = run_both(x, w, t, "none", torch.ones(T, device="cuda"), max_workspace=8 << 30)
+    rows = torch.cat([torch.arange(8), torch.arange(16738, 16746), torch.arange(T - 8, T)]).cuda()  # 2^31 falls into row 16743
+    out, ex, _, tol, bx, _ = formula(x[rows], w, t[rows], "none", torch.ones(len(rows), device="cuda"))
+    assert ((loss[rows].double() - out).abs() <= tol).all()
+    within(dx[rows], ex, bx, "dx")
+    cols = torch.cat([torch.arange(4), t[rows].cpu(), torch.tensor([V - 1])]).cuda()
+    want, size = torch.zeros(len(cols), H, dtype=torch.float64, device="cuda"), torch.zeros(len(cols), H, dtype=torch.float64, device="cuda")
+    for lo in range(0, T, 2000):
+        xs, ts = x[lo:lo + 2000].double(), t[lo:lo + 2000]
+        p = torch.softmax(xs @ w.double().t(), 1)[:, cols] - (ts[:, None] == cols).double()
+        want += p.t() @ xs
+        size += p.abs().t() @ xs.abs()
+    assert ((dw[cols].double() - want).abs() <= U * want.abs() + 4 * U * size).all()
+
+
+def test_more_rows_of_a_matrix_of_losses():
+    x, w, t = make(4 * 50, 64, 300, seed=14, ignored=0.2)
+    g = torch.rand(4, 50, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    xa, wa = x.detach().view(4, 50, 64).requires_grad_(), w.detach().requires_grad_()
+    (OF.linear_cross_entropy(xa, wa, t.view(4, 50), "none") * g).sum().backward()
+    _, dx, dw = run_both(x, w, t, "none", g.view(-1))
+    assert torch.equal(xa.grad.view(200, 64), dx) and torch.equal(wa.grad, dw)
+    # a gradient that is one number behind an expanded view
+    xb, wb = x.detach().requires_grad_(), w.detach().requires_grad_()
+    OF.linear_cross_entropy(xb, wb, t, "none").sum().backward()
+    _, dx, dw = run_both(x, w, t, "sum")
+    assert torch.equal(xb.grad, dx) and torch.equal(wb.grad, dw)
+
+
+def test_two_streams_at_once():
+    torch.cuda.synchronize()
+    work = []
+    for k in range(4):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            x, w, t = make(300 + 100 * k, 64, 500 + k, seed=40 + k)
+            work.append((s, x, w, t, run_both(x, w, t, "mean")))
+    torch.cuda.synchronize()
+    for s, x, w, t, got in work:
+        for a, b in zip(got, run_both(x, w, t, "mean")):
+            assert torch.equal(a, b)
+
+
+def test_status_word_read_between_forward_and_backward():
+    x, w, t = make(64, 64, 100)
+    x.requires_grad_()
+    loss = OF.linear_cross_entropy(x, w, t)
+    OF.status_word("cuda").zero_()
+    assert torch.isfinite(torch.autograd.grad(loss, x)[0]).all()
