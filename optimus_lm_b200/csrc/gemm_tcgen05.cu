@@ -12,7 +12,9 @@
 //                32 rows in 128B-swizzled shared memory and write them with cp.async.bulk.tensor stores (full
 //                128-byte lines) while the next tile's main loop runs; accumulating epilogues (C += A*B) use
 //                plain loads and stores.  With EPI_SWIGLU the tile holds 128 gate and 128 up columns of the same
-//                expert and the epilogue writes gate | up (for the backward) and w(row) * silu(gate) * up.
+//                expert and the epilogue writes gate | up (for the backward) and w(row) * silu(gate) * up.  EPI_CE
+//                (sixteen epilogue warps) writes exponentials of logits and their sums, see epilogue_ce; EPI_ROWSCALE
+//                multiplies each row by a factor of its own.
 //   * warps 6-9: only in the variants with a fused transfer (PeerArg<true>): all-gather of A's rows from the other
 //                GPUs, gather of the routed token rows into the expert-grouped operand (expert-parallel dispatch, or
 //                the local permutation on one GPU), or push of finished rows of C to their owners
@@ -90,6 +92,7 @@ struct GemmParams {
   const float* row_scale;      // EPI_ROWSCALE: row r of the product is multiplied by row_scale[r] before it is rounded
   // EPI_CE: see epilogue_ce.
   const long long* ce_targets;
+  int ce_v0, ce_v_total;       // B's rows are [ce_v0, ce_v0 + N) of a vocabulary of ce_v_total
   const float* ce_ref;
   unsigned* ce_max;
   float* ce_part;
@@ -159,7 +162,7 @@ __device__ __forceinline__ int stale_vectors_in_block(const PeerArg<true>& peers
 constexpr int STAGER_WARPS = 4;
 constexpr int NUM_THREADS_STAGED = NUM_THREADS + 32 * STAGER_WARPS;
 // Epilogue warps of a CTA and threads of a launch (EPI_CE: sixteen, see epilogue_ce).
-__host__ __device__ constexpr int epilogue_warps(int epi) { return epi == 4 ? 16 : 4; }
+__host__ __device__ constexpr int epilogue_warps(int epi) { return epi == EPI_CE ? 16 : 4; }
 __host__ __device__ constexpr int num_threads(bool peer, int epi) { return peer ? NUM_THREADS_STAGED : 64 + 32 * epilogue_warps(epi); }
 
 // Epilogue staging: each of the four epilogue warps owns two buffers of 32 rows x 128 bytes (what one tensor-map
@@ -595,9 +598,9 @@ __device__ __forceinline__ void epilogue_ce(const GemmParams& p, uint32_t stage,
   if (row0 >= p.M || x0 >= x_end) return;
   const bool row_ok = row < p.M;
   const long long target = row_ok ? p.ce_targets[row] : -1;
-  const bool live = target >= 0 && target < p.N;
+  const bool live = target >= 0 && target < p.ce_v_total;
   const bool all_live = __all_sync(0xffffffffu, live);
-  const int tcol = live ? static_cast<int>(target) - x0 : -1;
+  const int tcol = live ? static_cast<int>(target) - p.ce_v0 - x0 : -1;
   constexpr float LOG2E = 1.4426950408889634f;
   const float ref = live ? ce_row_ref(p, row) : 0.f;
   const float ref2 = ref * LOG2E;
@@ -1731,7 +1734,8 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   } else if (epi == OLB_EPI_CE) {
     // C = exponentials [M, N] (row stride ldc); dense, both operands K-major
     if (d->a_mn_major || d->b_mn_major || d->accumulate || d->out_fp32 || d->mode != OLB_GEMM_DENSE || d->n_peers ||
-        d->k_split || d->k_splits > 1 || d->ce_targets == nullptr || d->ce_ref == nullptr ||
+        d->k_split || d->k_splits > 1 || d->ce_v0 < 0 || (d->ce_v_total && d->ce_v_total < d->ce_v0 + d->N) ||
+        (d->ce_v_total == 0 && d->ce_v0) || d->ce_targets == nullptr || d->ce_ref == nullptr ||
         (d->ce_repair && (d->ce_flags == nullptr || d->ce_max == nullptr)) || (d->ce_flags != nullptr && d->ce_max == nullptr) ||
         (d->ce_part != nullptr && d->ce_part_ld < d->M))
       return -18;
@@ -1846,6 +1850,8 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   p.aux_out = d->aux_out;
   p.row_scale = d->row_scale;
   p.ce_targets = d->ce_targets;
+  p.ce_v0 = d->ce_v0;
+  p.ce_v_total = d->ce_v_total ? d->ce_v_total : d->N;
   p.ce_ref = d->ce_ref;
   p.ce_max = d->ce_max;
   p.ce_part = d->ce_part;

@@ -214,13 +214,18 @@ lce_finish_kernel(const olb_lce_finish_desc d) {
 
 __global__ void __launch_bounds__(LCE_THREADS)
 lce_patch_kernel(const float* __restrict__ prob, const long long* __restrict__ targets, int rows, int V,
-                 __nv_bfloat16* __restrict__ E, long long lde, float* __restrict__ factor) {
+                 const float* __restrict__ scale, float* __restrict__ factor, int v0, int cols, __nv_bfloat16* __restrict__ E,
+                 long long lde) {
   const int row = blockIdx.x * LCE_THREADS + threadIdx.x;
   if (row >= rows) return;
   const long long t = targets[row];
+  __nv_bfloat16 entry;
   float f = 0.f;
-  if (t >= 0 && t < V) f = lce_patch_row(E + row * lde + t, prob[row], 1.f);
-  factor[row] = f;
+  if (t >= 0 && t < V) {
+    f = lce_patch_row(&entry, prob[row], scale ? *scale : 1.f);
+    if (E && t >= v0 && t < v0 + cols) E[row * lde + (t - v0)] = entry;
+  }
+  if (factor) factor[row] = f;
 }
 
 // One warp per row.
@@ -273,7 +278,7 @@ lce_sum_parts_kernel(const float* __restrict__ part, int nparts, long long part_
 template <bool SRC_BF16, bool ACCUMULATE>
 __global__ void __launch_bounds__(LCE_THREADS)
 lce_scale_out_kernel(const void* __restrict__ src_, long long vecs, const float* __restrict__ grad, uint4* __restrict__ dst) {
-  const float g = grad ? *grad : 1.f;
+  const float g = *grad;
   for (long long i = blockIdx.x * static_cast<long long>(LCE_THREADS) + threadIdx.x; i < vecs;
        i += static_cast<long long>(gridDim.x) * LCE_THREADS) {
     float f[8];
@@ -340,11 +345,11 @@ extern "C" int olb_lce_finish(const olb_lce_finish_desc* d, cudaStream_t stream)
   return launch_waiting(lce_finish_kernel, (d->rows + LCE_ROWS - 1) / LCE_ROWS, stream, *d);
 }
 
-extern "C" int olb_lce_patch(const float* prob, const long long* targets, int rows, int V, void* E, long long lde,
-                             float* factor, cudaStream_t stream) {
+extern "C" int olb_lce_patch(const float* prob, const long long* targets, int rows, int V, const float* scale, float* factor,
+                             int v0, int cols, void* E, long long lde, cudaStream_t stream) {
   if (rows <= 0) return 0;
   lce_patch_kernel<<<(rows + LCE_THREADS - 1) / LCE_THREADS, LCE_THREADS, 0, stream>>>(
-      prob, targets, rows, V, static_cast<__nv_bfloat16*>(E), lde, factor);
+      prob, targets, rows, V, scale, factor, v0, cols, static_cast<__nv_bfloat16*>(E), lde);
   return launched();
 }
 

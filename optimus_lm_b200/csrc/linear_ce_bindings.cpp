@@ -1,13 +1,15 @@
 // Python bindings of the cross entropy from hidden states: the launch sequences of forward and backward.
 //
-// The batch is taken in pieces of rows whose exponentials [rows, V] (bf16) fit the caller's workspace limit.
-//   one piece, gradients wanted : forward = product + finish, exponentials and row factors are kept; backward = the two
-//                                 gradient products, straight to bf16 with the incoming gradient in the row factors.
-//   several pieces, one scalar  : the incoming gradient is a common factor, so forward runs the gradient products of
-//                                 each piece too (dX to bf16, dW summed in fp32) and backward scales; every logit is
-//                                 computed once (6 T H V operations in all).
-//   several pieces, loss per row: the rows' gradients are not known in the forward, which keeps two floats per row;
-//                                 backward computes the exponentials again (8 T H V operations).
+// The exponentials (bf16, [tokens, V]) are kept within the caller's workspace limit, in one of three ways:
+//   they fit                 : forward = product + finish, exponentials and row factors are kept; backward = the two
+//                              gradient products, straight to bf16 with the incoming gradient in the row factors.
+//   pieces of the batch      : for one scalar loss the incoming gradient is a common factor, so forward runs the gradient
+//                              products of each piece too (dX to bf16, dW summed in fp32) and backward scales them (one
+//                              more rounding of dX unless the gradient is a power of two); every logit is computed once, 6 T H V
+//                              operations in all.  Needs the fp32 dW within the limit as well.
+//   pieces of the vocabulary : losses per row, whose gradients the forward does not know, or a weight too large for the
+//                              fp32 dW.  Forward keeps two floats per row; backward computes the exponentials again, 8 T H V
+//                              operations in all, dX summed in fp32 over the pieces, dW's rows finished piece by piece.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -24,12 +26,12 @@ inline void check(int rc, const char* what) { TORCH_CHECK(rc == 0, std::string(w
 
 enum { MEAN = 0, SUM = 1, NONE = 2 };
 
-// What forward leaves to backward: with one piece the exponentials and row factors, with several the gradients of a
-// scalar loss (dx and dw in fp32; undefined where not wanted) or the rows' 1 - p_target and log-sum-exp.
+// What forward leaves to backward: the exponentials and row factors; or the gradients of a scalar loss (dx, and dw in
+// fp32; undefined where not wanted); or the rows' 1 - p_target and log-sum-exp and the count of the targets with its inverse.
 enum { PIECE = 0, SCALE = 1, AGAIN = 2 };
 struct Kept {
   int64_t kind = PIECE;
-  at::Tensor a, b;
+  at::Tensor a, b, c;
 };
 
 int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
@@ -84,21 +86,24 @@ int split_parts(int64_t M, int64_t N, int64_t K) {
   return best;
 }
 
-// e = exp(l - ref) of one piece (and the sums of its tiles), then the row blocks that need another reference.
-void product(const Problem& p, int64_t r0, int64_t rows, const float* ref, unsigned* top, int* flags, float* part,
-             int64_t part_ld, void* E, bool behind_prep) {
+// e = exp(l - ref) of some rows and columns [v0, v0 + cols) of the vocabulary (and the sums of their tiles), then of the
+// row blocks that need another reference.
+void product(const Problem& p, int64_t r0, int64_t rows, int64_t v0, int64_t cols, const float* ref, unsigned* top, int* flags,
+             float* part, int64_t part_ld, void* E, int64_t lde, bool behind_prep) {
   olb_gemm_desc d{};
   d.A = row_ptr(p.x, r0);
-  d.B = p.w.data_ptr();
+  d.B = row_ptr(p.w, v0);
   d.C = E;
   d.lda = p.x.stride(0);
   d.ldb = p.w.stride(0);
-  d.ldc = p.lde;
+  d.ldc = lde;
   d.a_rows = rows;
-  d.b_rows = p.V;
+  d.b_rows = cols;
   d.M = static_cast<int>(rows);
-  d.N = static_cast<int>(p.V);
+  d.N = static_cast<int>(cols);
   d.K = static_cast<int>(p.H);
+  d.ce_v0 = static_cast<int>(v0);
+  d.ce_v_total = static_cast<int>(p.V);
   d.epilogue = OLB_EPI_CE;
   d.status = p.status;
   d.ce_targets = ptr_i64(p.targets, r0);
@@ -154,27 +159,28 @@ void input_gradient(const Problem& p, int64_t r0, int64_t rows, const void* E, c
         "olb_lce_sum_parts");
 }
 
-// dw (=, += or, in fp32, reduced into) E^T xs
-void weight_gradient(const Problem& p, int64_t rows, const void* E, const void* xs, at::Tensor& dw, bool add) {
+// Rows [v0, v0 + cols) of dw (=, += or, in fp32, reduced into) E^T xs
+void weight_gradient(const Problem& p, int64_t rows, int64_t v0, int64_t cols, const void* E, int64_t lde, const void* xs,
+                     at::Tensor& dw, bool add) {
   olb_gemm_desc d{};
   d.A = E;
   d.B = xs;
-  d.C = dw.data_ptr();
-  d.lda = p.lde;
+  d.C = row_ptr(dw, v0);
+  d.lda = lde;
   d.ldb = p.H;
   d.ldc = dw.stride(0);
   d.a_rows = rows;
   d.b_rows = rows;
-  d.M = static_cast<int>(p.V);
+  d.M = static_cast<int>(cols);
   d.N = static_cast<int>(p.H);
   d.K = static_cast<int>(rows);
   d.a_mn_major = d.b_mn_major = 1;
   d.wide_tiles = 1;
   d.status = p.status;
   d.out_fp32 = dw.scalar_type() == at::kFloat;
-  const int parts = d.out_fp32 ? 1 : split_parts(p.V, p.H, rows);
+  const int parts = d.out_fp32 ? 1 : split_parts(cols, p.H, rows);
   if (parts > 1) {  // a small weight and a long batch
-    const int64_t part_rows = round_up(p.V, 128);
+    const int64_t part_rows = round_up(cols, 128);
     at::Tensor partial = at::empty({parts * part_rows, p.H}, p.x.options().dtype(at::kFloat));
     d.C = partial.data_ptr();
     d.ldc = p.H;
@@ -182,8 +188,8 @@ void weight_gradient(const Problem& p, int64_t rows, const void* E, const void* 
     d.k_splits = parts;
     d.c_part_rows = static_cast<int>(part_rows);
     check(olb_gemm_bf16(&d, p.stream), "olb_gemm_bf16 (weight gradient)");
-    check(olb_lce_sum_parts(partial.data_ptr<float>(), parts, part_rows, static_cast<int>(p.V), static_cast<int>(p.H), nullptr,
-                            dw.data_ptr(), add, p.stream),
+    check(olb_lce_sum_parts(partial.data_ptr<float>(), parts, part_rows, static_cast<int>(cols), static_cast<int>(p.H), nullptr,
+                            row_ptr(dw, v0), add, p.stream),
           "olb_lce_sum_parts");
     return;
   }
@@ -220,8 +226,8 @@ at::Tensor linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Ten
   }
   int64_t rows_max = piece_rows(p.T, grad ? 2 * p.lde : 4 * ((p.V + 15) / 16), max_bytes);
   const bool single = rows_max >= p.T;
-  const bool store = grad && (single || reduction != NONE);   // several pieces of losses per row: exponentials again later
-  if (grad && !single && reduction == NONE) rows_max = piece_rows(p.T, 4 * ((p.V + 15) / 16), max_bytes);
+  const bool store = grad && (single || (reduction != NONE && 4 * p.V * p.H <= max_bytes));
+  if (grad && !store) rows_max = piece_rows(p.T, 4 * ((p.V + 15) / 16), max_bytes);
   // sums per row, of whole pieces and of a shorter last one
   const int64_t last = p.T - (p.T - 1) / rows_max * rows_max;
   const int64_t ntiles_most = std::max(olb_gemm_ce_slices(static_cast<int>(std::min(rows_max, p.T)), static_cast<int>(p.V)),
@@ -231,12 +237,13 @@ at::Tensor linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Ten
   // small per-row and per-launch words: (losses,) ref, top, flags, ticket, count, 1 / count
   const int64_t losses = reduction == NONE ? 0 : p.T;
   at::Tensor words = at::empty({losses + 2 * rows_max + (rows_max + 127) / 128 + 1 + 3}, f32);
+  at::Tensor counts = grad && !store ? at::empty({2}, f32) : at::Tensor();  // outlives the words
   float* loss_rows = reduction == NONE ? out.data_ptr<float>() : words.data_ptr<float>();
   float* ref = words.data_ptr<float>() + losses;
   unsigned* top = reinterpret_cast<unsigned*>(ref + rows_max);
   int* flags = reinterpret_cast<int*>(top + rows_max);
   unsigned* ticket = reinterpret_cast<unsigned*>(flags + (rows_max + 127) / 128 + 1);
-  float* count = reinterpret_cast<float*>(ticket + 1);
+  float* count = counts.defined() ? counts.data_ptr<float>() : reinterpret_cast<float*>(ticket + 1);
   at::Tensor part = at::empty({ntiles_most, rows_max}, f32);
   at::Tensor E, factor, dx, dw32, prob, lse, xs;
   if (store) {
@@ -261,7 +268,7 @@ at::Tensor linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Ten
                        static_cast<int>(p.H), static_cast<int>(p.V), ref, top, flags, ticket, ptr_i64(p.targets, 0), p.T,
                        reduction == MEAN && r0 == 0 ? count : nullptr, p.stream),
           "olb_lce_prep");
-    product(p, r0, rows, ref, top, flags, part.data_ptr<float>(), rows_max, store ? E.data_ptr() : nullptr, true);
+    product(p, r0, rows, 0, p.V, ref, top, flags, part.data_ptr<float>(), rows_max, store ? E.data_ptr() : nullptr, p.lde, true);
     olb_lce_finish_desc f{};
     f.part = part.data_ptr<float>();
     f.part_ld = rows_max;
@@ -298,12 +305,12 @@ at::Tensor linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Ten
     check(olb_lce_finish(&f, p.stream), "olb_lce_finish");
     if (in_forward) {
       if (need_dx) input_gradient(p, r0, rows, E.data_ptr(), factor.data_ptr<float>(), dx, false);
-      if (need_dw) weight_gradient(p, rows, E.data_ptr(), xs.data_ptr(), dw32, r0 > 0);
+      if (need_dw) weight_gradient(p, rows, 0, p.V, E.data_ptr(), p.lde, xs.data_ptr(), dw32, r0 > 0);
     }
   }
   if (in_forward) kept = {SCALE, dx, dw32};
   else if (store) kept = {PIECE, E, factor};
-  else kept = {AGAIN, prob, lse};
+  else kept = {AGAIN, prob, lse, counts};
   return out;
 }
 
@@ -331,7 +338,7 @@ std::vector<at::Tensor> linear_ce_bwd(const at::Tensor& x, const at::Tensor& w, 
                            need_dw ? xs.data_ptr() : nullptr, p.stream),
         "olb_lce_scale_rows");
   if (need_dx) input_gradient(p, 0, p.T, E.data_ptr(), row_factor.data_ptr<float>(), dx, true);
-  if (need_dw) weight_gradient(p, p.T, E.data_ptr(), xs.data_ptr(), dw, accumulate);
+  if (need_dw) weight_gradient(p, p.T, 0, p.V, E.data_ptr(), p.lde, xs.data_ptr(), dw, accumulate);
   return {dx, dw};
 }
 
@@ -355,41 +362,67 @@ std::vector<at::Tensor> linear_ce_bwd_scale(const at::Tensor& dx_in, const at::T
   return {dx, dw};
 }
 
-// Several pieces of losses per row: exponentials against the known log-sum-exp, piece by piece.
+// Pieces of the vocabulary: exponentials against the known log-sum-exp.  counts: {count, 1 / count} for a mean.
 std::vector<at::Tensor> linear_ce_bwd_again(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets,
-                                            const at::Tensor& prob, const at::Tensor& lse, const at::Tensor& grad, bool need_dx,
-                                            bool need_dw, int64_t max_bytes, const c10::optional<at::Tensor>& dw_out,
-                                            bool accumulate, const at::Tensor& status) {
+                                            const at::Tensor& prob, const at::Tensor& lse, const at::Tensor& counts,
+                                            const at::Tensor& grad, bool mean, bool need_dx, bool need_dw, int64_t max_bytes,
+                                            const c10::optional<at::Tensor>& dw_out, bool accumulate, const at::Tensor& status) {
   c10::cuda::CUDAGuard guard(x.device());
   const Problem p = make_problem(x, w, targets, status);
-  TORCH_CHECK(grad.scalar_type() == at::kFloat && grad.device() == x.device() && grad.is_contiguous() && grad.numel() == p.T &&
-              prob.numel() == p.T && lse.numel() == p.T);
+  TORCH_CHECK(grad.scalar_type() == at::kFloat && grad.device() == x.device() && grad.is_contiguous() &&
+              (grad.dim() == 0 || grad.numel() == p.T) && prob.numel() == p.T && lse.numel() == p.T);
   const auto f32 = x.options().dtype(at::kFloat);
-  const int64_t rows_max = piece_rows(p.T, 2 * p.lde, max_bytes);
-  at::Tensor E = at::empty({rows_max, p.lde}, x.options());
-  at::Tensor factor = at::empty({rows_max}, f32), row_factor = at::empty({rows_max}, f32);
-  at::Tensor dx, dw, dw32, xs;
-  if (need_dx) dx = at::empty({p.T, p.H}, x.options());
+  const int64_t most = std::max<int64_t>(256, max_bytes / (2 * p.T) / 256 * 256);
+  const int64_t pieces = (p.V + most - 1) / most;
+  const int64_t cols_max = pieces == 1 ? p.V : round_up((p.V + pieces - 1) / pieces, 256), lde = round_up(cols_max, 64);
+  const int T = static_cast<int>(p.T), H = static_cast<int>(p.H), V = static_cast<int>(p.V);
+  at::Tensor E = at::empty({p.T, lde}, x.options());
+  at::Tensor factors = at::empty({2, p.T}, f32);
+  float *factor = factors.data_ptr<float>(), *row_factor = factor + p.T;
+  at::Tensor dx, dx32, dw, xs;
+  if (need_dx) dx32 = at::empty({p.T, p.H}, f32);
   if (need_dw) {
     dw = weight_gradient_out(p, dw_out, accumulate);
-    dw32 = at::empty({p.V, p.H}, f32);
-    xs = at::empty({rows_max, p.H}, x.options());
+    xs = at::empty({p.T, p.H}, x.options());
   }
-  for (int64_t r0 = 0; r0 < p.T; r0 += rows_max) {
-    const int64_t rows = std::min(rows_max, p.T - r0);
-    product(p, r0, rows, lse.data_ptr<float>() + r0, nullptr, nullptr, nullptr, 0, E.data_ptr(), false);
-    check(olb_lce_patch(prob.data_ptr<float>() + r0, ptr_i64(p.targets, r0), static_cast<int>(rows), static_cast<int>(p.V),
-                        E.data_ptr(), p.lde, factor.data_ptr<float>(), p.stream),
+  check(olb_lce_patch(prob.data_ptr<float>(), ptr_i64(p.targets, 0), T, V, mean ? counts.data_ptr<float>() + 1 : nullptr, factor, 0,
+                      0, nullptr, 0, p.stream),
+        "olb_lce_patch");
+  check(olb_lce_scale_rows(x.data_ptr(), x.stride(0), factor, grad.data_ptr<float>(), grad.dim() == 0 ? 0 : 1, T, H, row_factor,
+                           need_dw ? xs.data_ptr() : nullptr, p.stream),
+        "olb_lce_scale_rows");
+  for (int64_t v0 = 0; v0 < p.V; v0 += cols_max) {
+    const int64_t cols = std::min(cols_max, p.V - v0);
+    product(p, 0, p.T, v0, cols, lse.data_ptr<float>(), nullptr, nullptr, nullptr, 0, E.data_ptr(), lde, false);
+    check(olb_lce_patch(prob.data_ptr<float>(), ptr_i64(p.targets, 0), T, V, nullptr, nullptr, static_cast<int>(v0),
+                        static_cast<int>(cols), E.data_ptr(), lde, p.stream),
           "olb_lce_patch");
-    check(olb_lce_scale_rows(row_ptr(x, r0), x.stride(0), factor.data_ptr<float>(), grad.data_ptr<float>() + r0, 1,
-                             static_cast<int>(rows), static_cast<int>(p.H), row_factor.data_ptr<float>(),
-                             need_dw ? xs.data_ptr() : nullptr, p.stream),
-          "olb_lce_scale_rows");
-    if (need_dx) input_gradient(p, r0, rows, E.data_ptr(), row_factor.data_ptr<float>(), dx, false);
-    if (need_dw) weight_gradient(p, rows, E.data_ptr(), xs.data_ptr(), dw32, r0 > 0);
+    if (need_dx) {
+      olb_gemm_desc d{};
+      d.A = E.data_ptr();
+      d.B = row_ptr(p.w, v0);
+      d.C = dx32.data_ptr();
+      d.lda = lde;
+      d.ldb = p.w.stride(0);
+      d.ldc = p.H;
+      d.a_rows = p.T;
+      d.b_rows = cols;
+      d.M = T;
+      d.N = H;
+      d.K = static_cast<int>(cols);
+      d.b_mn_major = 1;
+      d.wide_tiles = 1;
+      d.status = p.status;
+      d.out_fp32 = 1;
+      d.c_reduce = v0 > 0;
+      check(olb_gemm_bf16(&d, p.stream), "olb_gemm_bf16 (input gradient)");
+    }
+    if (need_dw) weight_gradient(p, p.T, v0, cols, E.data_ptr(), lde, xs.data_ptr(), dw, accumulate);
   }
-  if (need_dw)
-    check(olb_lce_scale_out(dw32.data_ptr(), 0, dw32.numel(), nullptr, dw.data_ptr(), accumulate, p.stream), "olb_lce_scale_out");
+  if (need_dx) {
+    dx = at::empty({p.T, p.H}, x.options());
+    check(olb_lce_sum_parts(dx32.data_ptr<float>(), 1, p.T, T, H, row_factor, dx.data_ptr(), 0, p.stream), "olb_lce_sum_parts");
+  }
   return {dx, dw};
 }
 
@@ -415,7 +448,8 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
                             const at::Tensor& status, const c10::intrusive_ptr<GradHolder>& holder) {
     Kept kept;
     at::Tensor out = linear_ce_fwd(x, w, targets, reduction, need_dx, need_dw, max_bytes, status, kept);
-    ctx->save_for_backward({x, w, targets, kept.a, kept.b});
+    ctx->save_for_backward({x, w, targets, kept.a, kept.b, kept.c});
+    ctx->saved_data["mean"] = reduction == MEAN;
     ctx->saved_data["status"] = status;  // cleared in place by whoever reads it
     ctx->saved_data["kind"] = kept.kind;
     ctx->saved_data["need"] = static_cast<int64_t>(need_dx) + 2 * static_cast<int64_t>(need_dw);
@@ -438,11 +472,11 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
       into = holder->obj.attr("buf").cast<at::Tensor>();
       add = holder->obj.attr("ready").cast<bool>();
     }
-    const at::Tensor &x = saved[0], &w = saved[1], &targets = saved[2], &a = saved[3], &b = saved[4];
+    const at::Tensor &x = saved[0], &w = saved[1], &targets = saved[2], &a = saved[3], &b = saved[4], &c = saved[5];
     const at::Tensor status = ctx->saved_data["status"].toTensor();
     auto got = kind == PIECE   ? linear_ce_bwd(x, w, targets, a, b, grad, need_dx, need_dw, into, add, status)
                : kind == SCALE ? linear_ce_bwd_scale(a, b, grad, into, add)
-                               : linear_ce_bwd_again(x, w, targets, a, b, grad, need_dx, need_dw,
+                               : linear_ce_bwd_again(x, w, targets, a, b, c, grad, ctx->saved_data["mean"].toBool(), need_dx, need_dw,
                                                      ctx->saved_data["max_bytes"].toInt(), into, add, status);
     if (holder) {
       pybind11::gil_scoped_acquire gil;

@@ -105,7 +105,9 @@ typedef struct {
   // of olb_gemm_ce_slices(M, N) slices of the columns without the target's column.  ce_flags (may be NULL; 1 + ceil(M / 128) ints and ce_max M words, all
   // zero): a row whose largest logit exceeds its reference by more than 40 has it recorded in ce_max and its block of
   // 128 rows flagged.  ce_repair: the same product for the flagged blocks alone, rows with a recorded maximum against that.
+  // With ce_v_total, B holds rows [ce_v0, ce_v0 + N) of a vocabulary of that many and targets count in the whole of it.
   const long long* ce_targets;
+  int ce_v0, ce_v_total;
   const float* ce_ref;
   unsigned* ce_max;
   float* ce_part;
@@ -273,10 +275,10 @@ typedef struct {
 } olb_lce_finish_desc;
 // (launched so that it waits for the launch before it inside the kernel)
 int olb_lce_finish(const olb_lce_finish_desc* d, cudaStream_t stream);
-// The target entries of exponentials that were taken against the log-sum-exp: E[r, t] = -prob[r] (rounded), factor[r]
-// as above with the row's gradient grad[r * grad_stride].
-int olb_lce_patch(const float* prob, const long long* targets, int rows, int V, void* E, long long lde, float* factor,
-                  cudaStream_t stream);
+// For exponentials that were taken against the log-sum-exp: factor[r] as above (times *scale when that is not NULL; factor
+// may be NULL), and the target entries of the columns [v0, v0 + cols) in E (may be NULL): E[r, t - v0] = -prob[r] (rounded).
+int olb_lce_patch(const float* prob, const long long* targets, int rows, int V, const float* scale, float* factor, int v0,
+                  int cols, void* E, long long lde, cudaStream_t stream);
 // row_factor[r] = factor[r] * grad[r * grad_stride] and, when xs is not NULL, xs[r, :] = bf16(row_factor[r] * x[r, :]).
 // A product launched next with `overlap` starts under this.
 int olb_lce_scale_rows(const void* x, long long ldx, const float* factor, const float* grad, long long grad_stride, int rows,
@@ -285,7 +287,7 @@ int olb_lce_scale_rows(const void* x, long long ldx, const float* factor, const 
 // accumulate out[r, :] is added before the rounding).
 int olb_lce_sum_parts(const float* part, int nparts, long long part_rows, int rows, int H, const float* row_factor, void* out,
                       int accumulate, cudaStream_t stream);
-// dst (bf16) = (accumulate ? dst : 0) + *grad * src (NULL: 1), src fp32 or (src_bf16) bf16, n elements.
+// dst (bf16) = (accumulate ? dst : 0) + *grad * src, src fp32 or (src_bf16) bf16, n elements.
 int olb_lce_scale_out(const void* src, int src_bf16, long long n, const float* grad, void* dst, int accumulate,
                       cudaStream_t stream);
 

@@ -2,7 +2,7 @@
 optimus/kernels/*.py): time the tcgen05 GEMMs, the grouped expert GEMMs and flash attention
 against the library kernels with CUDA events, print TFLOP/s.
 
-    python -m optimus_lm_b200.ops.bench_kernels [gemm|grouped|attention|all]
+    python -m optimus_lm_b200.ops.bench_kernels [gemm|grouped|attention|loss|clip|all]
 """
 import sys
 
@@ -262,6 +262,54 @@ def profile_case(name: str, launches: int = 4):
     print(f"profile case {name}: {launches} launches done", flush=True)
 
 
+def bench_loss():
+    """Loss and gradients from the hidden states against the path over the logits: time and memory above the inputs."""
+    for B, S, H, V in [(4, 4096, 2048, 50304), (1, 4096, 7168, 129280), (16, 4096, 2048, 50304)]:
+        x = torch.randn(B, S, H, device="cuda").to(torch.bfloat16).requires_grad_()
+        w = (torch.randn(V, H, device="cuda") * 0.02).to(torch.bfloat16).requires_grad_()
+        labels = torch.randint(0, V, (B, S), device="cuda")
+
+        def logits_path():
+            return torch.autograd.grad(OF.shifted_cross_entropy(OF.linear(x, w), labels, inplace_backward=True), (x, w))
+
+        def hidden_path():
+            return torch.autograd.grad(OF.shifted_linear_cross_entropy(x, w, labels), (x, w))
+
+        msg = f"loss + gradients {B * S} x {H} against {V}:"
+        for label, fn in (("over the logits", logits_path), ("from the hidden states", hidden_path)):
+            t = _time(fn)
+            torch.cuda.reset_peak_memory_stats()
+            held = torch.cuda.memory_allocated()
+            fn()
+            torch.cuda.synchronize()
+            peak = (torch.cuda.max_memory_allocated() - held) / 2 ** 30
+            msg += f" {label} {t:.3f} ms ({6.0 * B * S * H * V / t * 1e-9:.0f} TFLOP/s, {peak:.2f} GiB) |"
+        print(msg, flush=True)
+        del x, w
+    assert OF.check_status("cuda") == 0
+
+
+def bench_clip():
+    """Norm and clipping of the gradients of a dense model (1.28e9 parameters, 147 tensors) against torch's utilities."""
+    sizes = [50304 * 2048] * 2 + ([2048 * 2048] * 4 + [2048] * 2 + [2048 * 8192] * 3) * 16 + [2048]
+    grads = [torch.randn(n, device="cuda").mul_(1e-3).to(torch.bfloat16) for n in sizes]
+    nbytes = 6 * sum(sizes)   # read for the norm, read and written for the scaling
+    limit = [1.0]
+
+    def ours():
+        limit[0] *= 0.99
+        OF.clip_grad_norm_(grads, limit[0])
+
+    def torch_utils():
+        limit[0] *= 0.99
+        norm = torch.nn.utils.get_total_norm(grads)
+        torch._foreach_mul_(grads, torch.clamp(limit[0] / (norm + 1e-6), max=1.0))
+
+    t1, t2 = _time(ours), _time(torch_utils)
+    print(f"clip {sum(sizes) / 1e9:.2f}e9 bf16 gradients in {len(sizes)} tensors: {t1:.3f} ms ({nbytes / t1 * 1e-6:.0f} GB/s) | "
+          f"torch {t2:.3f} ms", flush=True)
+
+
 if __name__ == "__main__":
     what = sys.argv[1] if len(sys.argv) > 1 else "all"
     if what.startswith("profile-"):
@@ -273,3 +321,7 @@ if __name__ == "__main__":
         bench_grouped()
     if what in ("attention", "all"):
         bench_attention()
+    if what in ("loss", "all"):
+        bench_loss()
+    if what in ("clip", "all"):
+        bench_clip()

@@ -980,9 +980,10 @@ def linear_cross_entropy(x, weight, targets, reduction="mean", max_workspace=1 <
     losses of the targets' shape.  The loss is fp32; gradients reach ``x`` and ``weight`` (once-differentiable).
 
     ``max_workspace`` bounds, in bytes, the exponentials of the logits held at a time (bf16, 2 V bytes for each
-    position); a batch that needs more is taken in pieces of positions.  With one piece the exponentials are kept until
-    the backward; with several, ``"mean"`` and ``"sum"`` compute the gradients in the forward (and need an fp32 ``[V, H]``
-    buffer), ``"none"`` computes the logits again in the backward.
+    position).  When those of all positions fit they are kept until the backward.  Otherwise ``"mean"`` and ``"sum"`` take
+    the batch in pieces and compute the gradients in the forward, if an fp32 ``[V, H]`` buffer fits the bound as well; if it
+    does not, and for ``"none"``, the backward computes the logits again in pieces of the vocabulary (a third more work,
+    and an fp32 buffer of ``x``'s shape).
 
     The kernel path takes bf16 CUDA tensors with ``H % 8 == 0``; other inputs take the plain one.  Reference: the
     ``lm_head`` of optimus/models/olmoe/modeling_olmoe.py:502-524 and ``F.cross_entropy`` on its logits."""
