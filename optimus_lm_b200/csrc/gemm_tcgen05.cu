@@ -83,13 +83,12 @@ struct GemmParams {
   const void* aux_in;
   long long aux_ld;
   float* aux_out;
-  // Dense mode, K range cut into k_splits parts of split_kb k-blocks each: part s writes its own partial product to rows
-  // [s * c_part_rows, + M) of C.  (Ragged-K: part = expert, c_part_rows = M.)
-  int k_splits, split_kb;
-  int c_part_rows;
+  // EPI_ROWSCALE: the tiles from tail_from on (the last, incomplete wave) are cut into tail_splits parts of tail_kb
+  // k-blocks each, which leave their fp32 products, tile after tile, to tail_sum_kernel.
+  int tail_from, tail_splits, tail_kb;
   int overlap;                 // the launch before this one may still be running: the epilogue waits for it
   int c_reduce;                // fp32 output added to C by the stores themselves (bulk reduction), no read in the kernel
-  const float* row_scale;      // EPI_ROWSCALE: row r of the product is multiplied by row_scale[r] before it is rounded
+  const float* row_scale;      // EPI_ROWSCALE, optional: row r of the product times row_scale[r] before it is rounded
   // EPI_CE: see epilogue_ce.
   const long long* ce_targets;
   int ce_v0, ce_v_total;       // B's rows are [ce_v0, ce_v0 + N) of a vocabulary of ce_v_total
@@ -184,15 +183,40 @@ struct TileInfo {
   int m0, n0;        // element offsets of the tile in C
   int kb_begin, kb_end;  // K range in units of BLOCK_K
   int expert;
+  int tail;              // EPI_ROWSCALE: 1 + the number of a part of a split tile, 0 for a whole tile
 };
 
-// K range of a dense or ragged-M tile: the whole of K, or part `part` of a split product.
-__device__ __forceinline__ void set_k_range(const GemmParams& p, int part, TileInfo& ti) {
+// Walk N fastest inside bands of 8 row blocks so that concurrently resident CTAs share operand tiles through L2.
+__device__ __forceinline__ void tile_blocks(int t, int num_m, int num_n, int& m_blk, int& n_blk) {
+  constexpr int BAND = 8;
+  const int band_tiles = BAND * num_n;
+  const int band = t / band_tiles;
+  const int first_m = band * BAND;
+  const int rows_in_band = min(BAND, num_m - first_m);
+  const int r = t - band * band_tiles;
+  m_blk = first_m + r % rows_in_band;
+  n_blk = r / rows_in_band;
+}
+
+// A launch's t-th piece of work when the tiles from p.tail_from on are split: `t` becomes the tile, `tail` 1 + the number
+// of its part among all parts (0: a whole tile).  The parts of one K range of all tail tiles follow each other.
+__device__ __forceinline__ bool split_tail(const GemmParams& p, int tiles, int& t, int& part, int& tail) {
+  part = tail = 0;
+  if (p.tail_splits > 1 && t >= p.tail_from) {
+    const int left = tiles - p.tail_from, u = t - p.tail_from;
+    part = u / left;
+    if (part >= p.tail_splits) return false;
+    t = p.tail_from + (u - part * left);
+    tail = 1 + (t - p.tail_from) * p.tail_splits + part;
+  }
+  return t < tiles;
+}
+__device__ __forceinline__ void set_k_range(const GemmParams& p, int part, int tail, TileInfo& ti) {
   ti.kb_begin = 0;
   ti.kb_end = (p.K + BLOCK_K - 1) / BLOCK_K;
-  if (p.k_splits > 1) {
-    ti.kb_begin = part * p.split_kb;
-    ti.kb_end = min(ti.kb_end, ti.kb_begin + p.split_kb);
+  if (tail) {
+    ti.kb_begin = part * p.tail_kb;
+    ti.kb_end = min(ti.kb_end, ti.kb_begin + p.tail_kb);
   }
 }
 
@@ -213,29 +237,20 @@ __device__ __forceinline__ bool get_tile(const GemmParams& p, int t, int num_m_b
     ti.kb_end = p.meta[e + 1] / BLOCK_K;
     return true;
   }
-  int part = 0;
-  if (p.k_splits > 1) {
-    part = t / (num_m_blocks * num_n_blocks);
-    if (part >= p.k_splits) return false;
-    t -= part * (num_m_blocks * num_n_blocks);
+  int part = 0, tail = 0;
+  if constexpr (EPI == EPI_ROWSCALE) {
+    if (!split_tail(p, num_m_blocks * num_n_blocks, t, part, tail)) return false;
   }
   if (t >= num_m_blocks * num_n_blocks) return false;
-  // Walk N fastest inside bands of 8 row blocks so that concurrently resident CTAs share
-  // operand tiles through L2.
-  constexpr int BAND = 8;
-  const int band_tiles = BAND * num_n_blocks;
-  const int band = t / band_tiles;
-  const int first_m = band * BAND;
-  const int rows_in_band = min(BAND, num_m_blocks - first_m);
-  const int r = t - band * band_tiles;
-  int m_blk = first_m + r % rows_in_band;
+  int m_blk, n_blk;
+  tile_blocks(t, num_m_blocks, num_n_blocks, m_blk, n_blk);
   if (p.m_rotate_blocks) m_blk = (m_blk + p.m_rotate_blocks) % num_m_blocks;
-  const int n_blk = r / rows_in_band;
   m_blk += blk0;  // first row block of the requested range
   ti.m0 = m_blk * BLOCK_M;
   ti.n0 = n_blk * TILE_N;
-  set_k_range(p, part, ti);
-  ti.expert = (p.mode == OLB_GEMM_RAGGED_M) ? p.meta[1 + m_blk] : part;
+  set_k_range(p, part, tail, ti);
+  ti.expert = (p.mode == OLB_GEMM_RAGGED_M) ? p.meta[1 + m_blk] : 0;
+  ti.tail = tail;
   return true;
 }
 
@@ -314,12 +329,12 @@ __device__ __forceinline__ void epilogue_plain(const GemmParams& p, const CUtens
   const int row = ti.m0 + lane_group * 32 + lane;
   const bool row_ok = row < p.M;
   float scale = 1.f;
-  if constexpr (ROWSCALE) scale = row_ok ? p.row_scale[row] : 0.f;
+  if constexpr (ROWSCALE) scale = row_ok && p.row_scale ? p.row_scale[row] : 1.f;
   if (p.c_tma) {
     // ---- staged tensor-map stores: 128 bytes of every row per turn (64 bf16 or 32 fp32 columns)
     long long y = ti.m0 + lane_group * 32;
     const bool rows_ok = y < p.M;
-    y += static_cast<long long>(ti.expert) * p.c_part_rows;
+    if (p.mode == OLB_GEMM_RAGGED_K) y += static_cast<long long>(ti.expert) * p.M;
     if (p.out_fp32) {
 #pragma unroll 1
       for (int c = 0; c < BLOCK_N / 32; ++c) {
@@ -429,6 +444,58 @@ __device__ __forceinline__ void epilogue_plain(const GemmParams& p, const CUtens
         }
       }
     }
+  }
+}
+
+// Epilogue of this warp's 32 rows of a split tile's part: the fp32 product as it is, to rows [y, y + 32) of the partial
+// products (tma_c2, BLOCK_N columns wide).
+template <int BLOCK_N>
+__device__ __forceinline__ void epilogue_tail(const GemmParams& p, const CUtensorMap* tma_c2, EpiStage& es, uint32_t taddr,
+                                              const TileInfo& ti, int y, int lane_group, int lane) {
+  if (ti.m0 + lane_group * 32 >= p.M) return;
+#pragma unroll 1
+  for (int c = 0; c < BLOCK_N / 32; ++c) {
+    if (ti.n0 + c * 32 >= p.N) break;
+    uint32_t r[32];
+    tmem_ld_32x32b_x32(taddr + c * 32, r);
+    tmem_ld_wait();
+    epi_store_chunk(es, tma_c2, r, lane, c * 32, y);
+  }
+}
+
+// The split tiles of a product with EPI_ROWSCALE: sum of a tile's parts in their order, times the row's factor, rounded once
+// into C (accumulate: added to it, in fp32).  8 columns per thread.
+__global__ void __launch_bounds__(256)
+tail_sum_kernel(const GemmParams p, const float* __restrict__ part, int num_m, int num_n, int tile_m, int tile_n) {
+  grid_dependency_wait();
+  const int vecs = tile_n / 8;
+  const long long a_tile = static_cast<long long>(tile_m) * tile_n;
+  const long long total = static_cast<long long>(num_m * num_n - p.tail_from) * tile_m * vecs;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const int q = static_cast<int>(i / (tile_m * vecs)), at = static_cast<int>(i - static_cast<long long>(q) * tile_m * vecs);
+    int m_blk, n_blk;
+    tile_blocks(p.tail_from + q, num_m, num_n, m_blk, n_blk);
+    const int row = m_blk * tile_m + at / vecs, col = n_blk * tile_n + at % vecs * 8;
+    if (row >= p.M || col >= p.N) continue;
+    const float4* src = reinterpret_cast<const float4*>(part + q * p.tail_splits * a_tile + at * 8ll);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+#pragma unroll 4
+    for (int s = 0; s < p.tail_splits; ++s) {
+      const float4 u = __ldcs(src + s * (a_tile / 4)), v = __ldcs(src + s * (a_tile / 4) + 1);
+      a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
+      b.x += v.x; b.y += v.y; b.z += v.z; b.w += v.w;
+    }
+    const float f = p.row_scale ? p.row_scale[row] : 1.f;
+    a.x *= f; a.y *= f; a.z *= f; a.w *= f;
+    b.x *= f; b.y *= f; b.z *= f; b.w *= f;
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.C) + row * p.ldc + col);
+    if (p.accumulate) {
+      const uint4 o = *dst;
+      const float2 c = unpack_bf16(o.x), d = unpack_bf16(o.y), e = unpack_bf16(o.z), g = unpack_bf16(o.w);
+      a.x += c.x; a.y += c.y; a.z += d.x; a.w += d.y;
+      b.x += e.x; b.y += e.y; b.z += g.x; b.w += g.y;
+    }
+    *dst = make_uint4(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w), pack_bf16(b.x, b.y), pack_bf16(b.z, b.w));
   }
 }
 
@@ -1076,7 +1143,12 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
       } else if constexpr (EPI == EPI_CE) {
         epilogue_ce<BLOCK_N>(p, smem_base + L::EPI_OFFSET + (warp - 2) * (EPI_BUF_BYTES / 2), taddr, ti, lane_group, (warp - 2) >> 2, lane);
       } else {
-        epilogue_plain<BLOCK_N, EPI == EPI_ROWSCALE>(p, &tma_c, es, taddr, ti, has_k, lane_group, lane);
+        bool part = false;
+        if constexpr (EPI == EPI_ROWSCALE) {
+          part = ti.tail != 0;
+          if (part) epilogue_tail<BLOCK_N>(p, &tma_c2, es, taddr, ti, (ti.tail - 1) * BLOCK_M + lane_group * 32, lane_group, lane);
+        }
+        if (!part) epilogue_plain<BLOCK_N, EPI == EPI_ROWSCALE>(p, &tma_c, es, taddr, ti, has_k, lane_group, lane);
       }
       if constexpr (PEER) {
         if (peers.push == 1 || peers.push == 2) {  // this warp's 32 rows of the tile are stored: let the stagers know
@@ -1150,25 +1222,19 @@ __device__ __forceinline__ bool get_tile_pair(const GemmParams& p, int t, int nu
     ti.kb_end = p.meta[e + 1] / BLOCK_K;
     return true;
   }
-  int part = 0;
-  if (p.k_splits > 1) {
-    part = t / (num_m * num_n);
-    if (part >= p.k_splits) return false;
-    t -= part * (num_m * num_n);
+  int part = 0, tail = 0;
+  if constexpr (EPI == EPI_ROWSCALE) {
+    if (!split_tail(p, num_m * num_n, t, part, tail)) return false;
   }
   if (t >= num_m * num_n) return false;
-  constexpr int BAND = 8;
-  const int band_tiles = BAND * num_n;
-  const int band = t / band_tiles;
-  const int first_m = band * BAND;
-  const int rows_in_band = min(BAND, num_m - first_m);
-  const int r = t - band * band_tiles;
-  const int m_pair = first_m + r % rows_in_band;
+  int m_pair, n_blk;
+  tile_blocks(t, num_m, num_n, m_pair, n_blk);
   ti.m0 = m_pair * 256;
-  ti.n0 = (r / rows_in_band) * TILE_N;
-  set_k_range(p, part, ti);
+  ti.n0 = n_blk * TILE_N;
+  set_k_range(p, part, tail, ti);
   // expert groups are padded to 256 rows (p.pair_rows), so both blocks of a pair belong to one expert
-  ti.expert = (p.mode == OLB_GEMM_RAGGED_M) ? p.meta[1 + 2 * m_pair] : part;
+  ti.expert = (p.mode == OLB_GEMM_RAGGED_M) ? p.meta[1 + 2 * m_pair] : 0;
+  ti.tail = tail;
   return true;
 }
 
@@ -1402,7 +1468,14 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
       } else if constexpr (EPI == EPI_CE) {
         epilogue_ce<BLOCK_N>(p, smem_base + L::EPI_OFFSET + (warp - 2) * (EPI_BUF_BYTES / 2), taddr, mine, lane_group, (warp - 2) >> 2, lane);
       } else {
-        epilogue_plain<BLOCK_N, EPI == EPI_ROWSCALE>(p, &tma_c, es, taddr, mine, has_k, lane_group, lane);
+        bool part = false;
+        if constexpr (EPI == EPI_ROWSCALE) {
+          part = ti.tail != 0;
+          if (part)
+            epilogue_tail<BLOCK_N>(p, &tma_c2, es, taddr, mine, (ti.tail - 1) * 256 + static_cast<int>(rank) * 128 + lane_group * 32,
+                                   lane_group, lane);
+        }
+        if (!part) epilogue_plain<BLOCK_N, EPI == EPI_ROWSCALE>(p, &tma_c, es, taddr, mine, has_k, lane_group, lane);
       }
       if constexpr (PEER) {
         if (peers.push == 1 || peers.push == 2) {  // this warp's 32 rows of the tile are stored: let the stagers know
@@ -1577,7 +1650,8 @@ static int launch(const TensorMaps& tm, const PeerArg<PEER>& peers, const GemmPa
   }
   const int TILE_N = EPI == EPI_SWIGLU ? BLOCK_N / 2 : (EPI == EPI_CE ? p.ce_tile_n : BLOCK_N);
   const long long nm = (p.M + BLOCK_M - 1) / BLOCK_M, nn = (p.N + TILE_N - 1) / TILE_N;
-  const long long tiles = nm * nn * (p.mode == OLB_GEMM_RAGGED_K ? p.num_experts : (p.k_splits > 1 ? p.k_splits : 1));
+  long long tiles = nm * nn * (p.mode == OLB_GEMM_RAGGED_K ? p.num_experts : 1);
+  if (EPI == EPI_ROWSCALE && p.tail_splits > 1) tiles = p.tail_from + (tiles - p.tail_from) * p.tail_splits;
   int grid = static_cast<int>(tiles < num_sms ? tiles : num_sms);
   if (grid <= 0) return 0;
   if constexpr (!PEER && (EPI == EPI_CE || EPI == EPI_PLAIN || EPI == EPI_ROWSCALE)) {
@@ -1605,7 +1679,8 @@ static int launch_pair(const TensorMaps& tm, const PeerArg<PEER>& peers, const G
   }
   constexpr int TILE_N = EPI == EPI_SWIGLU ? 128 : 256;
   const long long nm = (p.M + 255) / 256, nn = (p.N + TILE_N - 1) / TILE_N;
-  const long long tiles = nm * nn * (p.mode == OLB_GEMM_RAGGED_K ? p.num_experts : (p.k_splits > 1 ? p.k_splits : 1));
+  long long tiles = nm * nn * (p.mode == OLB_GEMM_RAGGED_K ? p.num_experts : 1);
+  if (EPI == EPI_ROWSCALE && p.tail_splits > 1) tiles = p.tail_from + (tiles - p.tail_from) * p.tail_splits;
   const int max_pairs = num_sms / 2;
   const int pairs = static_cast<int>(tiles < max_pairs ? tiles : max_pairs);
   if (pairs <= 0) return 0;
@@ -1697,12 +1772,75 @@ static CePlan ce_plan(int M, int N) {
   return best;
 }
 
+// Tiles of an EPI_ROWSCALE product and the split of its last wave.  Whole waves of tiles run as they are; the tiles that
+// would leave SMs idle in the last one are cut along K into as many parts as cost least: whole waves of parts at 1.5
+// PFLOP/s over the GPU, the parts' fp32 products written and read once at 4.5 TB/s, and 3 us for the launch that sums
+// them.  (4096 x 7168 against K = 129280: 448 tiles are six waves of 74 and four tiles, which take 18 parts each; splitting
+// every tile in four instead, for 25 waves of quarter tiles, moved 0.9 GB more and held 0.44 GiB.)
+struct RowscalePlan {
+  int block_n, pair, tile_m, num_m, num_n, tail_from, tail_splits, tail_kb;
+};
+static RowscalePlan rowscale_plan(const olb_gemm_desc* d, int sms) {
+  RowscalePlan r{};
+  r.block_n = d->N > 128 ? 256 : (d->N > 64 ? 128 : 64);
+  r.pair = pair_kernel_enabled() && r.block_n == 256 && d->M >= 256 && sms >= 2 &&
+           (d->N % 256 == 0 || d->N >= 2048 || (d->wide_tiles && (256 - d->N % 256) * 8 <= d->N));
+  r.tile_m = r.pair ? 256 : BLOCK_M;
+  r.num_m = (d->M + r.tile_m - 1) / r.tile_m;
+  r.num_n = (d->N + r.block_n - 1) / r.block_n;
+  const int workers = r.pair ? sms / 2 : sms, kb = (d->K + BLOCK_K - 1) / BLOCK_K;
+  const long long tiles = static_cast<long long>(r.num_m) * r.num_n;
+  const int left = static_cast<int>(tiles % workers);
+  r.tail_from = static_cast<int>(tiles - left);
+  r.tail_splits = 1;
+  if (left == 0) return r;
+  const double block_us = 2.0 * r.tile_m * r.block_n * BLOCK_K * workers / 1.5e9;
+  double least = 1e300;
+  for (int s = 1; s <= 148 && (s == 1 || kb / s >= 8); ++s) {
+    const int per = (kb + s - 1) / s;
+    if (static_cast<long long>(per) * (s - 1) >= kb) continue;  // an empty part
+    const double bytes = 8.0 * s * left * (d->M < r.tile_m ? d->M : r.tile_m) * r.block_n;
+    const double cost = (left * s + workers - 1) / workers * (per * block_us + 0.5) + (s > 1 ? bytes / 4.5e6 + 3.0 : 0.0);
+    if (cost < least) {
+      least = cost;
+      r.tail_splits = s;
+      r.tail_kb = per;
+    }
+  }
+  return r;
+}
+
 }  // namespace olb
 
 extern "C" int olb_gemm_ce_slices(int M, int N) {
   const olb::CePlan c = olb::ce_plan(M, N);
   const int cols = c.block_n / 4, full = N / c.tile_n, rest = N - full * c.tile_n;
   return full * ((c.tile_n + cols - 1) / cols) + (rest + cols - 1) / cols;
+}
+
+static int launch_tail_sum(const olb::RowscalePlan& r, const olb::GemmParams& p, const float* part, cudaStream_t stream) {
+  using namespace olb;
+  if (p.tail_splits <= 1) return 0;
+  const long long vecs = (static_cast<long long>(r.num_m) * r.num_n - r.tail_from) * r.tile_m * (r.block_n / 8);
+  const long long blocks = (vecs + 255) / 256;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;   // waits inside for the product
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, tail_sum_kernel, p, part, r.num_m, r.num_n, r.tile_m, r.block_n) == cudaSuccess ? 0 : -4;
+}
+
+extern "C" long long olb_gemm_tail_floats(const olb_gemm_desc* d) {
+  using namespace olb;
+  if (d->M <= 0 || d->N <= 0) return 0;
+  const RowscalePlan r = rowscale_plan(d, device_sm_count());
+  if (r.tail_splits <= 1) return 0;
+  return (static_cast<long long>(r.num_m) * r.num_n - r.tail_from) * r.tail_splits * r.tile_m * r.block_n;
 }
 
 extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
@@ -1715,6 +1853,7 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   const int epi = d->epilogue;
   int block_n = d->block_n;
   CePlan plan{0, 0, 0};
+  RowscalePlan tail{};
   if (epi == OLB_EPI_SWIGLU) {
     // N = width of act; B / B2 = gate / up weights (K-major, same layout); C = gate | up [rows, 2 N]; C2 = act [rows, N]
     if (d->N % 128 || d->B2 == nullptr || d->C2 == nullptr || d->b_mn_major || d->a_mn_major || d->accumulate ||
@@ -1734,7 +1873,7 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   } else if (epi == OLB_EPI_CE) {
     // C = exponentials [M, N] (row stride ldc); dense, both operands K-major
     if (d->a_mn_major || d->b_mn_major || d->accumulate || d->out_fp32 || d->mode != OLB_GEMM_DENSE || d->n_peers ||
-        d->k_split || d->k_splits > 1 || d->ce_v0 < 0 || (d->ce_v_total && d->ce_v_total < d->ce_v0 + d->N) ||
+        d->k_split || d->ce_v0 < 0 || (d->ce_v_total && d->ce_v_total < d->ce_v0 + d->N) ||
         (d->ce_v_total == 0 && d->ce_v0) || d->ce_targets == nullptr || d->ce_ref == nullptr ||
         (d->ce_repair && (d->ce_flags == nullptr || d->ce_max == nullptr)) || (d->ce_flags != nullptr && d->ce_max == nullptr) ||
         (d->ce_part != nullptr && d->ce_part_ld < d->M))
@@ -1742,10 +1881,12 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
     plan = ce_plan(d->M, d->N);
     block_n = plan.block_n;
   } else if (epi == OLB_EPI_ROWSCALE) {
-    if (d->row_scale == nullptr || d->accumulate || d->out_fp32 || d->mode != OLB_GEMM_DENSE || d->n_peers || d->k_splits > 1 ||
-        block_n != 0)
+    if ((d->accumulate && d->row_scale) || d->out_fp32 || d->mode != OLB_GEMM_DENSE || d->n_peers || block_n != 0 || d->max_ctas ||
+        (reinterpret_cast<uintptr_t>(d->tail_part) & 15))
       return -19;
-    block_n = d->N > 128 ? 256 : (d->N > 64 ? 128 : 64);
+    tail = rowscale_plan(d, device_sm_count());
+    if (d->tail_part == nullptr) tail.tail_splits = 1;
+    block_n = tail.block_n;
   } else if (epi != OLB_EPI_PLAIN) {
     return -12;
   } else if (block_n == 0) {
@@ -1863,22 +2004,15 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   p.ce_a_rows = a_box_rows;
   p.ce_grow = static_cast<float>(1.4426950408889634 * (1.0 + 1.4e-8 / 16 * d->K));
   p.ce_store = epi == OLB_EPI_CE && d->C != nullptr;
-  p.c_part_rows = d->mode == OLB_GEMM_RAGGED_K ? d->M : 0;
-  p.k_splits = 1;
-  if (d->k_splits > 1) {
-    // partial products of the K range, part s in rows [s * c_part_rows, + M) of an fp32 C; no part is empty
-    const int kb = (d->K + BLOCK_K - 1) / BLOCK_K;
-    const int per = (kb + d->k_splits - 1) / d->k_splits;
-    if (d->mode != OLB_GEMM_DENSE || epi != OLB_EPI_PLAIN || !d->out_fp32 || d->accumulate || d->n_peers || d->k_split ||
-        d->c_part_rows < d->M || d->c_part_rows % BLOCK_M || static_cast<long long>(per) * (d->k_splits - 1) >= kb)
-      return -20;
-    p.k_splits = d->k_splits;
-    p.split_kb = per;
-    p.b_expert_rows = 0;  // a part's number takes the expert's place in the tile
-    p.c_part_rows = d->c_part_rows;
+  p.tail_splits = 1;
+  if (epi == OLB_EPI_ROWSCALE) {
+    p.tail_from = tail.tail_from;
+    p.tail_splits = tail.tail_splits;
+    p.tail_kb = tail.tail_kb;
+    p.b_expert_rows = 0;
   }
   if (d->c_reduce) {
-    if (d->mode != OLB_GEMM_DENSE || epi != OLB_EPI_PLAIN || !d->out_fp32 || d->accumulate || d->n_peers || d->k_splits > 1)
+    if (d->mode != OLB_GEMM_DENSE || epi != OLB_EPI_PLAIN || !d->out_fp32 || d->accumulate || d->n_peers)
       return -21;
     p.c_reduce = 1;
   }
@@ -1901,7 +2035,7 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
     if (p.ce_store && d->ldc < (d->N + 63) / 64 * 64) return -18;  // whole chunks of 64 columns are written
   } else if (!d->accumulate) {
     const uint64_t esz = d->out_fp32 ? 4 : 2;
-    uint64_t rows = p.k_splits > 1 ? static_cast<uint64_t>(p.c_part_rows) * p.k_splits : d->M;
+    uint64_t rows = d->M;
     bool ok = (d->ldc * esz) % 16 == 0;
     if (d->mode == OLB_GEMM_RAGGED_K) {
       ok = ok && d->M % BLOCK_M == 0 && d->c_expert_stride == static_cast<long long>(d->M) * d->ldc;
@@ -1913,7 +2047,13 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
       p.c_tma = 1;
     }
   }
-  if ((p.k_splits > 1 || p.c_reduce || epi == OLB_EPI_ROWSCALE) && !p.c_tma) return -22;
+  if ((p.c_reduce || (epi == OLB_EPI_ROWSCALE && !d->accumulate)) && !p.c_tma) return -22;
+  if (p.tail_splits > 1) {
+    const uint64_t rows = (static_cast<uint64_t>(tail.num_m) * tail.num_n - tail.tail_from) * tail.tail_splits * tail.tile_m;
+    if (rows >= (1ull << 31)) return -20;
+    rc = make_tmap_2d(&tm.c2, d->tail_part, block_n, rows, block_n * 4ull, 32, 32, true);
+    if (rc) return rc;
+  }
 
   const int sms = d->max_ctas > 0 && d->max_ctas < num_sms ? d->max_ctas : num_sms;
   if (d->n_peers > 0) {
@@ -2025,10 +2165,14 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   if (use_pair) {
     if (epi == OLB_EPI_SWIGLU) return launch_pair<false, EPI_SWIGLU>(tm, nopeers, p, sms, stream);
     if (epi == OLB_EPI_SWIGLU_BWD) return launch_pair<false, EPI_SWIGLU_BWD>(tm, nopeers, p, sms, stream);
-    if (epi == OLB_EPI_ROWSCALE) return launch_pair<false, EPI_ROWSCALE>(tm, nopeers, p, sms, stream);
+    if (epi == OLB_EPI_ROWSCALE) {
+      rc = launch_pair<false, EPI_ROWSCALE>(tm, nopeers, p, sms, stream);
+      return rc ? rc : launch_tail_sum(tail, p, d->tail_part, stream);
+    }
     if (epi == OLB_EPI_CE) return launch_pair<false, EPI_CE>(tm, nopeers, p, sms, stream);
     return launch_pair<false, EPI_PLAIN>(tm, nopeers, p, sms, stream);
   }
   if (epi == OLB_EPI_SWIGLU_BWD) return -16;
-  return dispatch<false>(block_n, epi, tm, nopeers, p, sms, stream);
+  rc = dispatch<false>(block_n, epi, tm, nopeers, p, sms, stream);
+  return rc || epi != OLB_EPI_ROWSCALE ? rc : launch_tail_sum(tail, p, d->tail_part, stream);
 }

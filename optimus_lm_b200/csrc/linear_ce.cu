@@ -243,35 +243,18 @@ lce_scale_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, const 
   if (xs) lce_scale_row(x, ldx, xs, row, H, f, lane);
 }
 
-// 8 columns per thread; the parts are summed in their order.
-template <bool ACCUMULATE>
+// 8 columns per thread.
 __global__ void __launch_bounds__(LCE_THREADS)
-lce_sum_parts_kernel(const float* __restrict__ part, int nparts, long long part_rows, int rows, int H,
-                     const float* __restrict__ row_factor, __nv_bfloat16* __restrict__ out) {
-  grid_dependency_wait();
+lce_round_rows_kernel(const float4* __restrict__ src, int rows, int H, const float* __restrict__ row_factor,
+                      uint4* __restrict__ out) {
   const int vecs = H / 8;
   const long long total = static_cast<long long>(rows) * vecs;
   for (long long i = blockIdx.x * static_cast<long long>(LCE_THREADS) + threadIdx.x; i < total;
        i += static_cast<long long>(gridDim.x) * LCE_THREADS) {
-    const long long row = i / vecs;
-    const float4* src = reinterpret_cast<const float4*>(part + i * 8);
-    const long long step = part_rows * H / 4;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-#pragma unroll 4
-    for (int s = 0; s < nparts; ++s) {
-      const float4 u = __ldcs(src + s * step), v = __ldcs(src + s * step + 1);
-      a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
-      b.x += v.x; b.y += v.y; b.z += v.z; b.w += v.w;
-    }
-    const float f = row_factor ? row_factor[row] : 1.f;
-    if (ACCUMULATE) {  // (only without row factors)
-      const uint4 o = reinterpret_cast<const uint4*>(out)[i];
-      const float2 p = unpack_bf16(o.x), q = unpack_bf16(o.y), r = unpack_bf16(o.z), t = unpack_bf16(o.w);
-      a.x += p.x; a.y += p.y; a.z += q.x; a.w += q.y;
-      b.x += r.x; b.y += r.y; b.z += t.x; b.w += t.y;
-    }
-    reinterpret_cast<uint4*>(out)[i] = make_uint4(pack_bf16(f * a.x, f * a.y), pack_bf16(f * a.z, f * a.w),
-                                                  pack_bf16(f * b.x, f * b.y), pack_bf16(f * b.z, f * b.w));
+    const float4 a = __ldcs(src + 2 * i), b = __ldcs(src + 2 * i + 1);
+    const float f = row_factor[i / vecs];
+    out[i] = make_uint4(pack_bf16(f * a.x, f * a.y), pack_bf16(f * a.z, f * a.w), pack_bf16(f * b.x, f * b.y),
+                        pack_bf16(f * b.z, f * b.w));
   }
 }
 
@@ -362,14 +345,13 @@ extern "C" int olb_lce_scale_rows(const void* x, long long ldx, const float* fac
   return launched();
 }
 
-extern "C" int olb_lce_sum_parts(const float* part, int nparts, long long part_rows, int rows, int H, const float* row_factor,
-                                 void* out, int accumulate, cudaStream_t stream) {
-  if (H % 8 || misaligned(part) || misaligned(out) || nparts < 1 || (accumulate && row_factor)) return -1;
+extern "C" int olb_lce_round_rows(const float* src, int rows, int H, const float* row_factor, void* out, cudaStream_t stream) {
+  if (H % 8 || misaligned(src) || misaligned(out)) return -1;
   if (rows <= 0) return 0;
   const long long blocks = (static_cast<long long>(rows) * (H / 8) + LCE_THREADS - 1) / LCE_THREADS;
-  const int grid = static_cast<int>(blocks < 148 * 16 ? blocks : 148 * 16);
-  auto* kernel = accumulate ? lce_sum_parts_kernel<true> : lce_sum_parts_kernel<false>;
-  return launch_waiting(kernel, grid, stream, part, nparts, part_rows, rows, H, row_factor, static_cast<__nv_bfloat16*>(out));
+  lce_round_rows_kernel<<<static_cast<int>(blocks < 148 * 16 ? blocks : 148 * 16), LCE_THREADS, 0, stream>>>(
+      reinterpret_cast<const float4*>(src), rows, H, row_factor, static_cast<uint4*>(out));
+  return launched();
 }
 
 extern "C" int olb_lce_scale_out(const void* src, int src_bf16, long long n, const float* grad, void* dst, int accumulate,

@@ -63,27 +63,20 @@ int64_t piece_rows(int64_t T, int64_t bytes_per_row, int64_t max_bytes) {
 const long long* ptr_i64(const at::Tensor& t, int64_t at) { return reinterpret_cast<const long long*>(t.data_ptr<int64_t>()) + at; }
 void* row_ptr(const at::Tensor& t, int64_t row) { return static_cast<char*>(t.data_ptr()) + row * t.stride(0) * t.element_size(); }
 
-// Parts of the K range for C [M, N] += A [M, K] B: enough that the tiles fill the SMs, as few as possible.  Costs in
-// microseconds: a k-block of a tile at 1.5 PFLOP/s over the GPU, whole waves of tiles, and for more than one part the
-// fp32 partial products written and read once at 4.5 TB/s plus the launch that sums them.
-int split_parts(int64_t M, int64_t N, int64_t K) {
-  int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  const bool pair = M >= 256 && (N % 256 == 0 || N >= 2048 || (256 - N % 256) * 8 <= N);
-  const int64_t tm = pair ? 256 : 128, tn = N > 128 ? 256 : (N > 64 ? 128 : 64), workers = pair ? sms / 2 : sms;
-  const int64_t tiles = ((M + tm - 1) / tm) * ((N + tn - 1) / tn), kb = (K + 63) / 64;
-  const double block_us = 2.0 * tm * tn * 64 * workers / 1.5e9;
-  int best = 1;
-  double least = 1e30;
-  for (int s = 1; s <= 64 && (s == 1 || kb / s >= 8); ++s) {
-    const int64_t per = (kb + s - 1) / s;
-    if (per * (s - 1) >= kb) continue;
-    const double cost = ((tiles * s + workers - 1) / workers) * per * block_us + (s > 1 ? 8.0 * s * M * N / 4.5e6 + 4.0 : 0.0);
-    if (cost < least) {
-      least = cost;
-      best = s;
-    }
+// Runs an OLB_EPI_ROWSCALE product with the scratch that its last wave wants.
+void rowscale_product(const Problem& p, olb_gemm_desc& d, const char* what) {
+  d.epilogue = OLB_EPI_ROWSCALE;
+  d.wide_tiles = 1;
+  d.status = p.status;
+  const long long floats = olb_gemm_tail_floats(&d);
+  at::Tensor scratch;
+  if (floats > 0) {
+    scratch = at::empty({floats}, p.x.options().dtype(at::kFloat));
+    d.tail_part = scratch.data_ptr<float>();
+  } else if (d.row_scale == nullptr) {
+    d.epilogue = OLB_EPI_PLAIN;   // neither factors nor a split: 2 to 3 us less for 50304 x 2048
   }
-  return best;
+  check(olb_gemm_bf16(&d, p.stream), what);
 }
 
 // e = exp(l - ref) of some rows and columns [v0, v0 + cols) of the vocabulary (and the sums of their tiles), then of the
@@ -124,39 +117,22 @@ void product(const Problem& p, int64_t r0, int64_t rows, int64_t v0, int64_t col
 // dx[r0 .. r0 + rows) = row_factor * (E W).  behind_factors: the launch before it makes row_factor and not E.
 void input_gradient(const Problem& p, int64_t r0, int64_t rows, const void* E, const float* row_factor, at::Tensor& dx,
                     bool behind_factors) {
-  const int parts = split_parts(rows, p.H, p.V);
   olb_gemm_desc d{};
   d.A = E;
   d.B = p.w.data_ptr();
+  d.C = row_ptr(dx, r0);
   d.lda = p.lde;
   d.ldb = p.w.stride(0);
+  d.ldc = p.H;
   d.a_rows = rows;
   d.b_rows = p.V;
   d.M = static_cast<int>(rows);
   d.N = static_cast<int>(p.H);
   d.K = static_cast<int>(p.V);
   d.b_mn_major = 1;
-  d.wide_tiles = 1;
   d.overlap = behind_factors;
-  d.status = p.status;
-  d.ldc = p.H;
-  if (parts == 1) {
-    d.epilogue = OLB_EPI_ROWSCALE;
-    d.row_scale = row_factor;
-    d.C = row_ptr(dx, r0);
-    check(olb_gemm_bf16(&d, p.stream), "olb_gemm_bf16 (input gradient)");
-    return;
-  }
-  const int64_t part_rows = round_up(rows, 128);
-  at::Tensor partial = at::empty({parts * part_rows, p.H}, p.x.options().dtype(at::kFloat));
-  d.C = partial.data_ptr();
-  d.out_fp32 = 1;
-  d.k_splits = parts;
-  d.c_part_rows = static_cast<int>(part_rows);
-  check(olb_gemm_bf16(&d, p.stream), "olb_gemm_bf16 (input gradient)");
-  check(olb_lce_sum_parts(partial.data_ptr<float>(), parts, part_rows, static_cast<int>(rows), static_cast<int>(p.H),
-                          row_factor, row_ptr(dx, r0), 0, p.stream),
-        "olb_lce_sum_parts");
+  d.row_scale = row_factor;
+  rowscale_product(p, d, "olb_gemm_bf16 (input gradient)");
 }
 
 // Rows [v0, v0 + cols) of dw (=, += or, in fp32, reduced into) E^T xs
@@ -175,28 +151,15 @@ void weight_gradient(const Problem& p, int64_t rows, int64_t v0, int64_t cols, c
   d.N = static_cast<int>(p.H);
   d.K = static_cast<int>(rows);
   d.a_mn_major = d.b_mn_major = 1;
-  d.wide_tiles = 1;
-  d.status = p.status;
-  d.out_fp32 = dw.scalar_type() == at::kFloat;
-  const int parts = d.out_fp32 ? 1 : split_parts(cols, p.H, rows);
-  if (parts > 1) {  // a small weight and a long batch
-    const int64_t part_rows = round_up(cols, 128);
-    at::Tensor partial = at::empty({parts * part_rows, p.H}, p.x.options().dtype(at::kFloat));
-    d.C = partial.data_ptr();
-    d.ldc = p.H;
-    d.out_fp32 = 1;
-    d.k_splits = parts;
-    d.c_part_rows = static_cast<int>(part_rows);
-    check(olb_gemm_bf16(&d, p.stream), "olb_gemm_bf16 (weight gradient)");
-    check(olb_lce_sum_parts(partial.data_ptr<float>(), parts, part_rows, static_cast<int>(cols), static_cast<int>(p.H), nullptr,
-                            row_ptr(dw, v0), add, p.stream),
-          "olb_lce_sum_parts");
+  if (dw.scalar_type() == at::kBFloat16) {
+    d.accumulate = add;
+    rowscale_product(p, d, "olb_gemm_bf16 (weight gradient)");
     return;
   }
-  if (d.out_fp32)
-    d.c_reduce = add;
-  else
-    d.accumulate = add;
+  d.wide_tiles = 1;
+  d.status = p.status;
+  d.out_fp32 = 1;
+  d.c_reduce = add;
   check(olb_gemm_bf16(&d, p.stream), "olb_gemm_bf16 (weight gradient)");
 }
 
@@ -421,7 +384,7 @@ std::vector<at::Tensor> linear_ce_bwd_again(const at::Tensor& x, const at::Tenso
   }
   if (need_dx) {
     dx = at::empty({p.T, p.H}, x.options());
-    check(olb_lce_sum_parts(dx32.data_ptr<float>(), 1, p.T, T, H, row_factor, dx.data_ptr(), 0, p.stream), "olb_lce_sum_parts");
+    check(olb_lce_round_rows(dx32.data_ptr<float>(), T, H, row_factor, dx.data_ptr(), p.stream), "olb_lce_round_rows");
   }
   return {dx, dw};
 }

@@ -93,11 +93,12 @@ typedef struct {
   // (one int per 128 rows of B, zero at launch) counts the 16-byte vectors landed.  B is complete when the launch ends.
   const void* const* B_peers;
   const long long* b_seg;    // host array [2 * n_peers]
-  // Split K (DENSE, fp32 C): k_splits > 1 parts of whole 64-element blocks, none of them empty; part s is written to rows
-  // [s * c_part_rows, + M) of C (c_part_rows >= M, a multiple of 128), to be summed by the caller.
-  int k_splits, c_part_rows;
   int c_reduce;              // DENSE, fp32 C: C += A*B through reducing bulk stores (the kernel does not read C)
-  const float* row_scale;    // epilogue == OLB_EPI_ROWSCALE (DENSE, bf16 C): row r of the product times row_scale[r]
+  // epilogue == OLB_EPI_ROWSCALE (DENSE, bf16 C, written or without row_scale accumulated): row r of the product times
+  // row_scale[r] (NULL: 1).  With tail_part (olb_gemm_tail_floats(d) floats of scratch, 16-byte aligned) the tiles of an
+  // incomplete last wave are split along K and summed by a second launch.
+  const float* row_scale;
+  float* tail_part;
   // Cross-entropy product (epilogue == OLB_EPI_CE; DENSE, K-major operands): A = hidden states, B = the head's weight
   // [N, K] with any number of rows N.  Row r has its target in ce_targets[r] (outside [0, N): no target) and a reference
   // ce_ref[r]; with l the logits, C (may be NULL) receives exp(l - ref) as bf16, zeros for rows without a target and up to
@@ -123,6 +124,8 @@ typedef struct {
 } olb_gemm_desc;
 
 int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream);
+// Floats of scratch for tail_part (0: nothing to split).
+long long olb_gemm_tail_floats(const olb_gemm_desc* d);
 // Slices of N for which the cross-entropy product of M rows writes a sum of its own (at most ceil(N / 16) + 3).
 int olb_gemm_ce_slices(int M, int N);
 
@@ -283,10 +286,8 @@ int olb_lce_patch(const float* prob, const long long* targets, int rows, int V, 
 // A product launched next with `overlap` starts under this.
 int olb_lce_scale_rows(const void* x, long long ldx, const float* factor, const float* grad, long long grad_stride, int rows,
                        int H, float* row_factor, void* xs, cudaStream_t stream);
-// out[r, :] = bf16(row_factor[r] * sum_s part[s * part_rows + r, :]) in the order of s (row_factor NULL: 1, and then with
-// accumulate out[r, :] is added before the rounding).
-int olb_lce_sum_parts(const float* part, int nparts, long long part_rows, int rows, int H, const float* row_factor, void* out,
-                      int accumulate, cudaStream_t stream);
+// out[r, :] = bf16(row_factor[r] * src[r, :]), src fp32 [rows, H].
+int olb_lce_round_rows(const float* src, int rows, int H, const float* row_factor, void* out, cudaStream_t stream);
 // dst (bf16) = (accumulate ? dst : 0) + *grad * src, src fp32 or (src_bf16) bf16, n elements.
 int olb_lce_scale_out(const void* src, int src_bf16, long long n, const float* grad, void* dst, int accumulate,
                       cudaStream_t stream);

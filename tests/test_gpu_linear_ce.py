@@ -431,3 +431,45 @@ def test_status_word_read_between_forward_and_backward():
     loss = OF.linear_cross_entropy(x, w, t)
     OF.status_word("cuda").zero_()
     assert torch.isfinite(torch.autograd.grad(loss, x)[0]).all()
+
+
+@pytest.mark.parametrize("T,H,V", [(300, 1000, 3000), (512, 2048, 20000), (2500, 2048, 600), (1000, 256, 30), (40, 4096, 5000), (19000, 264, 100),
+                                   (3000, 2304, 300)])
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_products_whose_last_wave_is_split(T, H, V, reduction):
+    # gradients of more, and of fewer, tiles than the GPU has processors, long in the vocabulary or in the batch
+    x, w, t = make(T, H, V, seed=50, ignored=0.1)
+    check(x, w, t, reduction)
+
+
+def test_split_products_into_the_flat_gradient_buffer():
+    x, w, t = make(6000, 264, 100, seed=51)
+    _, _, dw = run_both(x, w, t, "mean")
+    w = torch.nn.Parameter(w)
+    w.grad = torch.zeros_like(w)
+    OF.enable_direct_grads([w])
+    for _ in range(2):
+        OF.linear_cross_entropy(x, w, t).backward()
+    want = dw.float() + dw.float()
+    assert ((w.grad.float() - want).abs() <= 2 * U * want.abs() + 2 * U * dw.float().abs() + 1e-30).all()
+
+
+@pytest.mark.parametrize("reduction,way", [("mean", "columns"), ("none", "columns"), ("mean", "rows")])
+def test_memory_stays_in_bounds(reduction, way):
+    T, H, V = 8192, 256, 20000   # exponentials of 328 MB
+    x, w, t = make(T, H, V, seed=52)
+    x.requires_grad_(), w.requires_grad_()
+    bound = 4 * w.numel() - (way == "columns")   # with or without room for the fp32 gradient of the weight
+    OF.linear_cross_entropy(x[:256], w, t[:256], "sum").backward()
+    x.grad = w.grad = None
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    loss = OF.linear_cross_entropy(x, w, t, reduction, max_workspace=bound)
+    torch.autograd.grad(loss, (x, w), torch.ones_like(loss))
+    torch.cuda.synchronize()
+    peak = torch.cuda.max_memory_allocated() - held
+    # the exponentials and (rows) the weight's fp32 gradient or (columns) the fp32 one of x, both gradients, scaled rows, and
+    # what splits a product's last wave: at most 148 tiles of 128 x 256 in fp32 a part
+    most = 2 * bound + 4 * x.numel() + 2 * (x.numel() * 2 + w.numel()) + 148 * 128 * 256 * 4 * 2 + (8 << 20)
+    assert peak <= most < 2 * T * V, (peak, most)
