@@ -136,6 +136,7 @@ lce_finish_kernel(const olb_lce_finish_desc d) {
   constexpr int TILES = LCE_THREADS / LCE_ROWS;
   __shared__ float s_sum[TILES][LCE_ROWS];
   __shared__ float s_factor[LCE_ROWS];
+  __shared__ double s_total[LCE_WARPS];
   __shared__ bool s_last;
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -198,17 +199,18 @@ lce_finish_kernel(const olb_lce_finish_desc d) {
   __syncthreads();
   if (!s_last) return;
   __threadfence();
-  float acc = 0.f;
+  double acc = 0.0;  // a long batch has many losses of one sign
 #pragma unroll 16
   for (long long i = threadIdx.x; i < d.n_all; i += LCE_THREADS) acc += __ldcg(d.loss_all + i);
-  acc = warp_sum(acc);
-  if (lane == 0) s_factor[warp] = acc;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+  if (lane == 0) s_total[warp] = acc;
   __syncthreads();
   if (threadIdx.x == 0) {
-    float sum = 0.f;
-    for (int i = 0; i < LCE_WARPS; ++i) sum += s_factor[i];
+    double sum = 0.0;
+    for (int i = 0; i < LCE_WARPS; ++i) sum += s_total[i];
     // a division, as a mean is defined: 0 / 0 where no row has a target
-    *d.total = d.total_scale ? sum / *d.total_scale : sum;
+    *d.total = static_cast<float>(d.total_scale ? sum / *d.total_scale : sum);
   }
 }
 
