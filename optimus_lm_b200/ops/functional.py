@@ -984,6 +984,8 @@ def linear_cross_entropy(x, weight, targets, reduction="mean", max_workspace=1 <
     the batch in pieces and compute the gradients in the forward, if an fp32 ``[V, H]`` buffer fits the bound as well; if it
     does not, and for ``"none"``, the backward computes the logits again in pieces of the vocabulary (a third more work,
     and an fp32 buffer of ``x``'s shape).
+    (16384 tokens x 2048 against 50304, peak memory above the inputs and time: 2 GiB allowed 1.87 GiB, 7.4 to 7.9 ms; 1 GiB
+    1.29 GiB, 7.8 to 8.1; 512 MiB 0.91 GiB, 8.3; 128 MiB 0.57 GiB, 10.7; over the logits 1.79 GiB, 7.5.)
 
     The kernel path takes bf16 CUDA tensors with ``H % 8 == 0``; other inputs take the plain one.  Reference: the
     ``lm_head`` of optimus/models/olmoe/modeling_olmoe.py:502-524 and ``F.cross_entropy`` on its logits."""
