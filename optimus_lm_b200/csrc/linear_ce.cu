@@ -130,11 +130,12 @@ __device__ __forceinline__ float lce_patch_row(__nv_bfloat16* entry, float S, fl
 
 // Block: 8 rows (a 32-byte sector of every tile's sums) x 32 tiles at a time; eight threads finish the rows, then each
 // warp scales one row of X.  (32 rows per block left half of the SMs without one: 29 us for 8192 x 2048, V = 50304.)
-constexpr int LCE_ROWS = 8;
+// With few rows one per block (one row of 2292 sums: 7 us with eight).
+template <int LCE_ROWS>
 __global__ void __launch_bounds__(LCE_THREADS)
 lce_finish_kernel(const olb_lce_finish_desc d) {
   constexpr int TILES = LCE_THREADS / LCE_ROWS;
-  __shared__ float s_sum[TILES][LCE_ROWS];
+  __shared__ float s_sum[LCE_WARPS][LCE_ROWS];
   __shared__ float s_factor[LCE_ROWS];
   __shared__ double s_total[LCE_WARPS];
   __shared__ bool s_last;
@@ -151,7 +152,9 @@ lce_finish_kernel(const olb_lce_finish_desc d) {
 #pragma unroll 8
       for (int i = threadIdx.x / LCE_ROWS; i < d.ntiles; i += TILES) s += p[i * d.part_ld];
     }
-    s_sum[threadIdx.x / LCE_ROWS][sub] = s;
+#pragma unroll
+    for (int o = 16; o >= LCE_ROWS; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane < LCE_ROWS) s_sum[warp][sub] = s;
   }
   __syncthreads();
   if (threadIdx.x < LCE_ROWS) {
@@ -161,7 +164,7 @@ lce_finish_kernel(const olb_lce_finish_desc d) {
       if (t >= 0 && t < d.V) {
         float S = 0.f;
 #pragma unroll
-        for (int i = 0; i < TILES; ++i) S += s_sum[i][sub];
+        for (int i = 0; i < LCE_WARPS; ++i) S += s_sum[i][sub];
         const float lt = d.ref[row];
         const unsigned m = d.ce_max[row];
         float z;
@@ -188,8 +191,8 @@ lce_finish_kernel(const olb_lce_finish_desc d) {
   }
   __syncthreads();
   if (d.xs) {
-    static_assert(LCE_WARPS == LCE_ROWS, "one warp per row");
-    if (row0 + warp < d.rows) lce_scale_row(d.x, d.ldx, d.xs, row0 + warp, d.H, s_factor[warp], lane);
+    static_assert(LCE_ROWS <= LCE_WARPS, "a warp per row");
+    if (warp < LCE_ROWS && row0 + warp < d.rows) lce_scale_row(d.x, d.ldx, d.xs, row0 + warp, d.H, s_factor[warp], lane);
   }
   if (d.total == nullptr) return;
   // the last block to arrive sums the rows' losses, in a fixed order
@@ -327,7 +330,8 @@ extern "C" int olb_lce_prep(const void* x, long long ldx, const void* w, long lo
 extern "C" int olb_lce_finish(const olb_lce_finish_desc* d, cudaStream_t stream) {
   if ((d->xs && (d->H % 8 || d->ldx % 8 || misaligned(d->x) || misaligned(d->xs))) || (d->total && !d->ticket)) return -1;
   if (d->rows <= 0) return 0;
-  return launch_waiting(lce_finish_kernel, (d->rows + LCE_ROWS - 1) / LCE_ROWS, stream, *d);
+  if (d->rows <= 148 * 2) return launch_waiting(lce_finish_kernel<1>, d->rows, stream, *d);
+  return launch_waiting(lce_finish_kernel<8>, (d->rows + 7) / 8, stream, *d);
 }
 
 extern "C" int olb_lce_patch(const float* prob, const long long* targets, int rows, int V, const float* scale, float* factor,
