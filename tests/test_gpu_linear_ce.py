@@ -473,3 +473,21 @@ def test_memory_stays_in_bounds(reduction, way):
     # what splits a product's last wave: at most 148 tiles of 128 x 256 in fp32 a part
     most = 2 * bound + 4 * x.numel() + 2 * (x.numel() * 2 + w.numel()) + 148 * 128 * 256 * 4 * 2 + (8 << 20)
     assert peak <= most < 2 * T * V, (peak, most)
+
+
+@pytest.mark.parametrize("T,H,V", [(5, 64, 300), (300, 264, 777), (1100, 136, 301)])
+@pytest.mark.parametrize("way", WAYS)
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_nothing_is_read_that_was_not_written(T, H, V, way, reduction):
+    # workspaces come from memory that held NaN
+    x, w, t = make(T, H, V, seed=60, ignored=0.2)
+    g = torch.rand(T, device="cuda") if reduction == "none" else None
+    want = run_both(x, w, t, reduction, g, **limit(way, w))
+    sizes = [2 * T * V, 4 * V * H, 2 * V * H, 4 * T * H, 2 * T * H, 64 * T, 4 * T, 1 << 21, 1 << 24]
+    for _ in range(2):
+        poison = [torch.full((n // 4 + 64,), float("nan"), device="cuda") for n in sizes for _ in range(3)]
+        torch.cuda.synchronize()
+        del poison
+        got = run_both(x, w, t, reduction, g, **limit(way, w))
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
