@@ -1158,6 +1158,8 @@ def _grad_norm_reference(grads, norm_type):
 
 def _check_grads(grads, norm_type):
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    if grads and not isinstance(grads[0], torch.Tensor):
+        raise TypeError("gradients must be tensors")   # the others are looked at where they are read
     if norm_type not in (2, math.inf):
         raise ValueError(f"norm_type must be 2 or inf, not {norm_type!r}")
     return grads
@@ -1178,6 +1180,8 @@ def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
         norm = extension().grad_clip(grads, norm_type == math.inf, False, 0.0, 0.0)
         if norm is not None:
             return norm
+    if not all(isinstance(g, torch.Tensor) for g in grads):
+        raise TypeError("gradients must be tensors")
     if any(g.device != grads[0].device for g in grads):
         raise ValueError("the gradients are on different devices")
     grads = [g for g in grads if g.numel()]

@@ -43,3 +43,12 @@ def test_refusals():
     with pytest.raises(ValueError):
         OF.grad_norm([torch.ones(3), torch.ones(3, device="meta")])
     assert torch.equal(g[0], torch.ones(3))
+
+
+@pytest.mark.parametrize("bad", [[None], [torch.ones(3), None], [1.0], [torch.ones(3), [torch.ones(3)]]])
+def test_only_tensors(bad):
+    with pytest.raises(TypeError):
+        OF.grad_norm(bad)
+    with pytest.raises(TypeError):
+        OF.clip_grad_norm_(bad, 1.0)
+    assert not isinstance(bad[0], torch.Tensor) or torch.equal(bad[0], torch.ones(3))
