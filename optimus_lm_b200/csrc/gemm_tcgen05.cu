@@ -97,7 +97,6 @@ struct GemmParams {
   float* ce_part;
   long long ce_part_ld;
   int* ce_flags;               // [0] any row block flagged, [1 + b] row block b (128 rows) flagged
-  float ce_grow;               // see epilogue_ce
   int ce_a_rows;               // rows of A in a tile's boxes: 128, or fewer in a launch of one row block
   int ce_tile_n;               // columns per tile, a multiple of 32 up to BLOCK_N
   int ce_repair;               // only the flagged row blocks, with their rows' recorded maxima as references
@@ -636,16 +635,16 @@ __device__ __forceinline__ bool ce_skip_tile(const GemmParams& p, const TileInfo
 // Epilogue of one 128-row tile of the cross-entropy product: the accumulator holds the logits l of the row against
 // vocabulary columns [ti.n0, ti.n0 + BLOCK_N).  With the row's reference m (its target's logit, or a log-sum-exp that
 // is known already) it writes e = exp(l - m) as bf16 to C (ce_store) and the row's sum of e over half a tile without
-// the target's column to ce_part[half tile][row].  exp is taken of fp32 values as 2^(l c - m log2e), one multiply-add
+// the target's column to ce_part[half tile][row].  exp is taken of fp32 values as 2^(l log2e - m log2e), one multiply-add
 // and one exponential for a logit; the rounding of m log2e is common to a row and goes back into its sum.  Nothing is
 // rounded to fewer bits before that, and e keeps bf16's relative precision however small it is.  Columns past N and
 // rows without a target give zeros.  A row whose sum shows a logit more than CE_RANGE above the reference has its
 // largest logit recorded in ce_max and its row block flagged; a second launch (ce_repair) computes those blocks again
 // against the recorded maxima.
-// The tensor cores truncate as they add: against the exact sum a logit of H terms of random sign comes out smaller by
-// 1.4e-8 of itself for every 16 terms (measured: 4.0e-7 at H = 512, 1.8e-6 at 2048, 6.9e-6 at 7168; up to 6e-8 where all
-// terms have one sign), and a mean loss would keep that bias.  c = ce_grow = log2e (1 + 1.4e-8 H / 16) gives it back,
-// which halves the logits' rms error (2.1e-6 to 1.1e-6 at H = 2048).
+// The logits are what the tensor cores sum.  These truncate as they add, towards zero: sums of H terms of random sign come
+// out smaller by 1.4e-8 of themselves for every 16 terms (measured: 4.0e-7 at H = 512, 1.8e-6 at 2048, 6.9e-6 at 7168), sums
+// of one sign by up to 6e-8, sums without anything to round not at all.  No factor gives that back for all of them (the
+// first one's, 1 + 1.4e-8 H / 16, is an error of 6e-6 for a logit that comes from a few of 7168 channels): none is applied.
 // CE_RANGE: sums of 2^31 terms of e^40 = 2.4e17 stay below 1e27, far inside fp32 and bf16, and so does their inverse.
 //
 // Sixteen warps per CTA work on a tile: each four take a quarter of its columns (a warp's dependent instructions leave
@@ -674,7 +673,7 @@ __device__ __forceinline__ void epilogue_ce(const GemmParams& p, uint32_t stage,
   // 2^(ref2 - ref log2e), to be given back: the product's rounding and that of the constant (LOG2E = log2e + 1.9e-8 log2e)
   const float slip = (fmaf(-ref, LOG2E, ref2) + ref * 2.7e-8f) * 0.6931472f;
   const float2 neg_ref2 = make_float2(-ref2, -ref2);
-  const float2 grow = make_float2(p.ce_grow, p.ce_grow);
+  const float2 log2e = make_float2(LOG2E, LOG2E);
   const uint32_t cols = taddr + part * COLS;
   float2 sum = make_float2(0.f, 0.f);
   // this lane's part of the coalesced stores: rows lane / UNITS + k * ROWS, 16-byte unit lane % UNITS
@@ -699,7 +698,7 @@ __device__ __forceinline__ void epilogue_ce(const GemmParams& p, uint32_t stage,
     }
 #pragma unroll
     for (int i = 0; i < CHUNK / 2; ++i) {
-      const float2 d = fma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), grow, neg_ref2);
+      const float2 d = fma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), log2e, neg_ref2);
       r[2 * i] = __float_as_uint(ex2_approx(d.x));
       r[2 * i + 1] = __float_as_uint(ex2_approx(d.y));
     }
@@ -2002,7 +2001,6 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   p.overlap = d->overlap;
   p.ce_tile_n = plan.tile_n;
   p.ce_a_rows = a_box_rows;
-  p.ce_grow = static_cast<float>(1.4426950408889634 * (1.0 + 1.4e-8 / 16 * d->K));
   p.ce_store = epi == OLB_EPI_CE && d->C != nullptr;
   p.tail_splits = 1;
   if (epi == OLB_EPI_ROWSCALE) {
