@@ -635,9 +635,10 @@ __device__ __forceinline__ bool ce_skip_tile(const GemmParams& p, const TileInfo
 // Epilogue of one 128-row tile of the cross-entropy product: the accumulator holds the logits l of the row against
 // vocabulary columns [ti.n0, ti.n0 + BLOCK_N).  With the row's reference m (its target's logit, or a log-sum-exp that
 // is known already) it writes e = exp(l - m) as bf16 to C (ce_store) and the row's sum of e over half a tile without
-// the target's column to ce_part[half tile][row].  exp is taken of fp32 values as 2^(l log2e - m log2e), one multiply-add
-// and one exponential for a logit; the rounding of m log2e is common to a row and goes back into its sum.  Nothing is
-// rounded to fewer bits before that, and e keeps bf16's relative precision however small it is.  Columns past N and
+// the target's column to ce_part[half tile][row].  exp is taken of fp32 values as 2^((l - m) log2e): the
+// difference first, which is exact for logits near the reference however large both are.  (One multiply-add less per logit
+// as 2^(l log2e - m log2e), but the rounding of m log2e, common to the row, is 4 % of e at m = 2^20.)  Nothing is rounded to
+// fewer bits before that, and e keeps bf16's relative precision however small it is.  Columns past N and
 // rows without a target give zeros.  A row whose sum shows a logit more than CE_RANGE above the reference has its
 // largest logit recorded in ce_max and its row block flagged; a second launch (ce_repair) computes those blocks again
 // against the recorded maxima.
@@ -669,10 +670,7 @@ __device__ __forceinline__ void epilogue_ce(const GemmParams& p, uint32_t stage,
   const int tcol = live ? static_cast<int>(target) - p.ce_v0 - x0 : -1;
   constexpr float LOG2E = 1.4426950408889634f;
   const float ref = live ? ce_row_ref(p, row) : 0.f;
-  const float ref2 = ref * LOG2E;
-  // 2^(ref2 - ref log2e), to be given back: the product's rounding and that of the constant (LOG2E = log2e + 1.9e-8 log2e)
-  const float slip = (fmaf(-ref, LOG2E, ref2) + ref * 2.7e-8f) * 0.6931472f;
-  const float2 neg_ref2 = make_float2(-ref2, -ref2);
+  const float2 neg_ref = make_float2(-ref, -ref);
   const float2 log2e = make_float2(LOG2E, LOG2E);
   const uint32_t cols = taddr + part * COLS;
   float2 sum = make_float2(0.f, 0.f);
@@ -698,7 +696,7 @@ __device__ __forceinline__ void epilogue_ce(const GemmParams& p, uint32_t stage,
     }
 #pragma unroll
     for (int i = 0; i < CHUNK / 2; ++i) {
-      const float2 d = fma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), log2e, neg_ref2);
+      const float2 d = mul2(add2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), neg_ref), log2e);
       r[2 * i] = __float_as_uint(ex2_approx(d.x));
       r[2 * i + 1] = __float_as_uint(ex2_approx(d.y));
     }
@@ -735,7 +733,7 @@ __device__ __forceinline__ void epilogue_ce(const GemmParams& p, uint32_t stage,
       }
     }
   }
-  const float total = (sum.x + sum.y) * (1.f + slip);
+  const float total = sum.x + sum.y;
   const int slice = ti.n0 / p.ce_tile_n * ((p.ce_tile_n + COLS - 1) / COLS) + part;
   if (live && p.ce_part) p.ce_part[static_cast<long long>(slice) * p.ce_part_ld + row] = total;
   if (p.ce_flags == nullptr || p.ce_repair) return;

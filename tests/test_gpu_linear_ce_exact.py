@@ -82,3 +82,16 @@ def test_wide_hidden_states_of_few_channels(H, way):
     T = 3000 if way == "rows" else 600
     check(*problem(H, torch.arange(1.0, 17.0), 1.0, T), "mean", way)
     check(*problem(H, torch.arange(1.0, 17.0), 1.0, T), "none", way)
+
+# logits of up to 992 and of 2^20 to 2^21, of both signs
+LARGE = {"hundreds": (torch.cat([torch.arange(1.0, 63.0), -torch.arange(1.0, 63.0)]), 16.0),
+         "millions": (torch.cat([torch.arange(1024.0, 2048.0, 8.0), -torch.arange(1024.0, 2048.0, 8.0)]), 1024.0)}
+
+
+@pytest.mark.parametrize("way", ["whole", "rows"])
+@pytest.mark.parametrize("size", LARGE)
+@pytest.mark.parametrize("far", [False, True])
+def test_large_logits(size, far, way):
+    check(*problem(16, *LARGE[size], far=far), "mean", way)
+    if way == "whole":
+        check(*problem(16, *LARGE[size], far=far), "none", way)
