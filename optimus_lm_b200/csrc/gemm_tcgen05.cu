@@ -633,7 +633,7 @@ __device__ __forceinline__ bool ce_skip_tile(const GemmParams& p, const TileInfo
 }
 
 // Epilogue of one 128-row tile of the cross-entropy product: the accumulator holds the logits l of the row against
-// vocabulary columns [ti.n0, ti.n0 + BLOCK_N).  With the row's reference m (its target's logit, or a log-sum-exp that
+// vocabulary columns [ti.n0, ti.n0 + BLOCK_N).  With the row's reference m (its target's logit, or a maximum that
 // is known already) it writes e = exp(l - m) as bf16 to C (ce_store) and the row's sum of e over half a tile without
 // the target's column to ce_part[half tile][row].  exp is taken of fp32 values as 2^((l - m) log2e): the
 // difference first, which is exact for logits near the reference however large both are.  (One multiply-add less per logit

@@ -160,7 +160,7 @@ lce_finish_kernel(const olb_lce_finish_desc d) {
   if (threadIdx.x < LCE_ROWS) {
     float factor = 0.f;
     if (ok) {
-      float loss = 0.f, prob = 0.f, lse = 0.f;
+      float loss = 0.f, sum = 0.f, base = 0.f, inv_z = 0.f;
       if (t >= 0 && t < d.V) {
         float S = 0.f;
 #pragma unroll
@@ -171,20 +171,23 @@ lce_finish_kernel(const olb_lce_finish_desc d) {
         if (m == 0) {  // the exponentials are relative to the target's logit
           z = 1.f + S;
           loss = log1pf(S);
+          base = lt;
         } else {       // ... to the row's maximum
-          const float top = __uint_as_float((m & 0x80000000u) ? (m & 0x7fffffffu) : ~m);
-          z = S + expf(lt - top);
-          loss = logf(z) + (top - lt);
+          base = __uint_as_float((m & 0x80000000u) ? (m & 0x7fffffffu) : ~m);
+          z = S + expf(lt - base);
+          loss = logf(z) + (base - lt);
         }
-        lse = lt + loss;
-        prob = S / z;
-        float inv_z = 1.f / z;
+        sum = S;
+        inv_z = 1.f / z;
         if (d.scale) inv_z *= *d.scale;
         if (d.E) factor = lce_patch_row(static_cast<__nv_bfloat16*>(d.E) + row * d.lde + t, S, inv_z);
       }
       d.loss[row] = loss;
-      if (d.prob) d.prob[row] = prob;
-      if (d.lse) d.lse[row] = lse;
+      if (d.sum) {
+        d.sum[row] = sum;
+        d.base[row] = base;
+        d.inv_z[row] = inv_z;
+      }
       if (d.factor) d.factor[row] = factor;
     }
     s_factor[sub] = factor;
@@ -218,16 +221,15 @@ lce_finish_kernel(const olb_lce_finish_desc d) {
 }
 
 __global__ void __launch_bounds__(LCE_THREADS)
-lce_patch_kernel(const float* __restrict__ prob, const long long* __restrict__ targets, int rows, int V,
-                 const float* __restrict__ scale, float* __restrict__ factor, int v0, int cols, __nv_bfloat16* __restrict__ E,
-                 long long lde) {
+lce_patch_kernel(const float* __restrict__ sum, const float* __restrict__ inv_z, const long long* __restrict__ targets, int rows,
+                 int V, float* __restrict__ factor, int v0, int cols, __nv_bfloat16* __restrict__ E, long long lde) {
   const int row = blockIdx.x * LCE_THREADS + threadIdx.x;
   if (row >= rows) return;
   const long long t = targets[row];
   __nv_bfloat16 entry;
   float f = 0.f;
   if (t >= 0 && t < V) {
-    f = lce_patch_row(&entry, prob[row], scale ? *scale : 1.f);
+    f = lce_patch_row(&entry, sum[row], inv_z[row]);
     if (E && t >= v0 && t < v0 + cols) E[row * lde + (t - v0)] = entry;
   }
   if (factor) factor[row] = f;
@@ -328,17 +330,19 @@ extern "C" int olb_lce_prep(const void* x, long long ldx, const void* w, long lo
 }
 
 extern "C" int olb_lce_finish(const olb_lce_finish_desc* d, cudaStream_t stream) {
-  if ((d->xs && (d->H % 8 || d->ldx % 8 || misaligned(d->x) || misaligned(d->xs))) || (d->total && !d->ticket)) return -1;
+  if ((d->xs && (d->H % 8 || d->ldx % 8 || misaligned(d->x) || misaligned(d->xs))) || (d->total && !d->ticket) ||
+      (d->sum && (!d->base || !d->inv_z)))
+    return -1;
   if (d->rows <= 0) return 0;
   if (d->rows <= 148 * 2) return launch_waiting(lce_finish_kernel<1>, d->rows, stream, *d);
   return launch_waiting(lce_finish_kernel<8>, (d->rows + 7) / 8, stream, *d);
 }
 
-extern "C" int olb_lce_patch(const float* prob, const long long* targets, int rows, int V, const float* scale, float* factor,
+extern "C" int olb_lce_patch(const float* sum, const float* inv_z, const long long* targets, int rows, int V, float* factor,
                              int v0, int cols, void* E, long long lde, cudaStream_t stream) {
   if (rows <= 0) return 0;
   lce_patch_kernel<<<(rows + LCE_THREADS - 1) / LCE_THREADS, LCE_THREADS, 0, stream>>>(
-      prob, targets, rows, V, scale, factor, v0, cols, static_cast<__nv_bfloat16*>(E), lde);
+      sum, inv_z, targets, rows, V, factor, v0, cols, static_cast<__nv_bfloat16*>(E), lde);
   return launched();
 }
 

@@ -8,7 +8,8 @@
 //                              more rounding of dX unless the gradient is a power of two); every logit is computed once, 6 T H V
 //                              operations in all.  Needs the fp32 dW within the limit as well.
 //   pieces of the vocabulary : losses per row, whose gradients the forward does not know, or a weight too large for the
-//                              fp32 dW.  Forward keeps two floats per row; backward computes the exponentials again, 8 T H V
+//                              fp32 dW.  Forward keeps three floats per row (what its exponentials were relative to, their
+//                              sum, 1 / Z); backward computes the same exponentials again, 8 T H V
 //                              operations in all, dX summed in fp32 over the pieces, dW's rows finished piece by piece.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -27,11 +28,11 @@ inline void check(int rc, const char* what) { TORCH_CHECK(rc == 0, std::string(w
 enum { MEAN = 0, SUM = 1, NONE = 2 };
 
 // What forward leaves to backward: the exponentials and row factors; or the gradients of a scalar loss (dx, and dw in
-// fp32; undefined where not wanted); or the rows' 1 - p_target and log-sum-exp and the count of the targets with its inverse.
+// fp32; undefined where not wanted); or the rows' sum, 1 / Z and reference, as [3, T].
 enum { PIECE = 0, SCALE = 1, AGAIN = 2 };
 struct Kept {
   int64_t kind = PIECE;
-  at::Tensor a, b, c;
+  at::Tensor a, b;
 };
 
 int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
@@ -200,15 +201,14 @@ at::Tensor linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Ten
   // small per-row and per-launch words: (losses,) ref, top, flags, ticket, count, 1 / count
   const int64_t losses = reduction == NONE ? 0 : p.T;
   at::Tensor words = at::empty({losses + 2 * rows_max + (rows_max + 127) / 128 + 1 + 3}, f32);
-  at::Tensor counts = grad && !store ? at::empty({2}, f32) : at::Tensor();  // outlives the words
   float* loss_rows = reduction == NONE ? out.data_ptr<float>() : words.data_ptr<float>();
   float* ref = words.data_ptr<float>() + losses;
   unsigned* top = reinterpret_cast<unsigned*>(ref + rows_max);
   int* flags = reinterpret_cast<int*>(top + rows_max);
   unsigned* ticket = reinterpret_cast<unsigned*>(flags + (rows_max + 127) / 128 + 1);
-  float* count = counts.defined() ? counts.data_ptr<float>() : reinterpret_cast<float*>(ticket + 1);
+  float* count = reinterpret_cast<float*>(ticket + 1);
   at::Tensor part = at::empty({ntiles_most, rows_max}, f32);
-  at::Tensor E, factor, dx, dw32, prob, lse, xs;
+  at::Tensor E, factor, dx, dw32, stats, xs;
   if (store) {
     E = at::empty({rows_max, p.lde}, x.options());
     factor = at::empty({rows_max}, f32);
@@ -221,10 +221,7 @@ at::Tensor linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Ten
       xs = at::empty({rows_max, p.H}, x.options());
     }
   }
-  if (grad && !store) {
-    prob = at::empty({p.T}, f32);
-    lse = at::empty({p.T}, f32);
-  }
+  if (grad && !store) stats = at::empty({3, p.T}, f32);
   for (int64_t r0 = 0; r0 < p.T; r0 += rows_max) {
     const int64_t rows = std::min(rows_max, p.T - r0);
     check(olb_lce_prep(row_ptr(x, r0), x.stride(0), w.data_ptr(), w.stride(0), ptr_i64(p.targets, r0), static_cast<int>(rows),
@@ -243,16 +240,17 @@ at::Tensor linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Ten
     f.V = static_cast<int>(p.V);
     f.H = static_cast<int>(p.H);
     f.loss = loss_rows + r0;
-    if (prob.defined()) {
-      f.prob = prob.data_ptr<float>() + r0;
-      f.lse = lse.data_ptr<float>() + r0;
+    if (stats.defined()) {
+      f.sum = stats.data_ptr<float>() + r0;
+      f.inv_z = f.sum + p.T;
+      f.base = f.inv_z + p.T;
     }
     if (store) {
       f.E = E.data_ptr();
       f.lde = p.lde;
       f.factor = factor.data_ptr<float>();
-      f.scale = reduction == MEAN ? count + 1 : nullptr;
     }
+    if (grad) f.scale = reduction == MEAN ? count + 1 : nullptr;
     if (xs.defined()) {
       f.x = row_ptr(x, r0);
       f.ldx = x.stride(0);
@@ -273,7 +271,7 @@ at::Tensor linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Ten
   }
   if (in_forward) kept = {SCALE, dx, dw32};
   else if (store) kept = {PIECE, E, factor};
-  else kept = {AGAIN, prob, lse, counts};
+  else kept = {AGAIN, stats};
   return out;
 }
 
@@ -325,15 +323,16 @@ std::vector<at::Tensor> linear_ce_bwd_scale(const at::Tensor& dx_in, const at::T
   return {dx, dw};
 }
 
-// Pieces of the vocabulary: exponentials against the known log-sum-exp.  counts: {count, 1 / count} for a mean.
+// Pieces of the vocabulary: the forward's exponentials again, against the references that it recorded.
 std::vector<at::Tensor> linear_ce_bwd_again(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets,
-                                            const at::Tensor& prob, const at::Tensor& lse, const at::Tensor& counts,
-                                            const at::Tensor& grad, bool mean, bool need_dx, bool need_dw, int64_t max_bytes,
-                                            const c10::optional<at::Tensor>& dw_out, bool accumulate, const at::Tensor& status) {
+                                            const at::Tensor& stats, const at::Tensor& grad, bool need_dx, bool need_dw,
+                                            int64_t max_bytes, const c10::optional<at::Tensor>& dw_out, bool accumulate,
+                                            const at::Tensor& status) {
   c10::cuda::CUDAGuard guard(x.device());
   const Problem p = make_problem(x, w, targets, status);
   TORCH_CHECK(grad.scalar_type() == at::kFloat && grad.device() == x.device() && grad.is_contiguous() &&
-              (grad.dim() == 0 || grad.numel() == p.T) && prob.numel() == p.T && lse.numel() == p.T);
+              (grad.dim() == 0 || grad.numel() == p.T) && stats.is_contiguous() && stats.numel() == 3 * p.T);
+  const float *sum = stats.data_ptr<float>(), *inv_z = sum + p.T, *base = inv_z + p.T;
   const auto f32 = x.options().dtype(at::kFloat);
   const int64_t most = std::max<int64_t>(256, max_bytes / (2 * p.T) / 256 * 256);
   const int64_t pieces = (p.V + most - 1) / most;
@@ -348,17 +347,15 @@ std::vector<at::Tensor> linear_ce_bwd_again(const at::Tensor& x, const at::Tenso
     dw = weight_gradient_out(p, dw_out, accumulate);
     xs = at::empty({p.T, p.H}, x.options());
   }
-  check(olb_lce_patch(prob.data_ptr<float>(), ptr_i64(p.targets, 0), T, V, mean ? counts.data_ptr<float>() + 1 : nullptr, factor, 0,
-                      0, nullptr, 0, p.stream),
-        "olb_lce_patch");
+  check(olb_lce_patch(sum, inv_z, ptr_i64(p.targets, 0), T, V, factor, 0, 0, nullptr, 0, p.stream), "olb_lce_patch");
   check(olb_lce_scale_rows(x.data_ptr(), x.stride(0), factor, grad.data_ptr<float>(), grad.dim() == 0 ? 0 : 1, T, H, row_factor,
                            need_dw ? xs.data_ptr() : nullptr, p.stream),
         "olb_lce_scale_rows");
   for (int64_t v0 = 0; v0 < p.V; v0 += cols_max) {
     const int64_t cols = std::min(cols_max, p.V - v0);
-    product(p, 0, p.T, v0, cols, lse.data_ptr<float>(), nullptr, nullptr, nullptr, 0, E.data_ptr(), lde, false);
-    check(olb_lce_patch(prob.data_ptr<float>(), ptr_i64(p.targets, 0), T, V, nullptr, nullptr, static_cast<int>(v0),
-                        static_cast<int>(cols), E.data_ptr(), lde, p.stream),
+    product(p, 0, p.T, v0, cols, base, nullptr, nullptr, nullptr, 0, E.data_ptr(), lde, false);
+    check(olb_lce_patch(sum, inv_z, ptr_i64(p.targets, 0), T, V, nullptr, static_cast<int>(v0), static_cast<int>(cols), E.data_ptr(),
+                        lde, p.stream),
           "olb_lce_patch");
     if (need_dx) {
       olb_gemm_desc d{};
@@ -411,8 +408,7 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
                             const at::Tensor& status, const c10::intrusive_ptr<GradHolder>& holder) {
     Kept kept;
     at::Tensor out = linear_ce_fwd(x, w, targets, reduction, need_dx, need_dw, max_bytes, status, kept);
-    ctx->save_for_backward({x, w, targets, kept.a, kept.b, kept.c});
-    ctx->saved_data["mean"] = reduction == MEAN;
+    ctx->save_for_backward({x, w, targets, kept.a, kept.b});
     ctx->saved_data["status"] = status;  // cleared in place by whoever reads it
     ctx->saved_data["kind"] = kept.kind;
     ctx->saved_data["need"] = static_cast<int64_t>(need_dx) + 2 * static_cast<int64_t>(need_dw);
@@ -435,12 +431,12 @@ struct LinearCE : torch::autograd::Function<LinearCE> {
       into = holder->obj.attr("buf").cast<at::Tensor>();
       add = holder->obj.attr("ready").cast<bool>();
     }
-    const at::Tensor &x = saved[0], &w = saved[1], &targets = saved[2], &a = saved[3], &b = saved[4], &c = saved[5];
+    const at::Tensor &x = saved[0], &w = saved[1], &targets = saved[2], &a = saved[3], &b = saved[4];
     const at::Tensor status = ctx->saved_data["status"].toTensor();
     auto got = kind == PIECE   ? linear_ce_bwd(x, w, targets, a, b, grad, need_dx, need_dw, into, add, status)
                : kind == SCALE ? linear_ce_bwd_scale(a, b, grad, into, add)
-                               : linear_ce_bwd_again(x, w, targets, a, b, c, grad, ctx->saved_data["mean"].toBool(), need_dx, need_dw,
-                                                     ctx->saved_data["max_bytes"].toInt(), into, add, status);
+                               : linear_ce_bwd_again(x, w, targets, a, grad, need_dx, need_dw, ctx->saved_data["max_bytes"].toInt(),
+                                                     into, add, status);
     if (holder) {
       pybind11::gil_scoped_acquire gil;
       holder->obj.attr("ready") = true;

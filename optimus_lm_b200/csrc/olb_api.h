@@ -251,7 +251,8 @@ int olb_lce_prep(const void* x, long long ldx, const void* w, long long ldw, con
                  int V, float* ref, unsigned* ce_max, int* ce_flags, unsigned* ticket, const long long* all_targets,
                  long long n_all, float* count, cudaStream_t stream);
 // Sums ce_part over its `ntiles` tiles and writes per row loss[r] (0 without a target) and, when they are not NULL,
-// prob[r] = 1 - p_target, lse[r], and with E (the exponentials, row stride lde): the target's entry of E, and
+// sum[r] (of the exponentials without the target's), base[r] (what they are relative to) and inv_z[r] = 1 / (sum and the
+// target's), and with E (the exponentials, row stride lde): the target's entry of E, and
 // factor[r] such that factor[r] * E[r, :] is the row's gradient (times *scale when scale is not NULL); xs (may be NULL):
 // bf16(factor[r] * x[r, :]).  total (may be NULL): sum of loss_all[0, n_all) times *total_scale (NULL: 1), taken by
 // the last block through *ticket.
@@ -263,7 +264,7 @@ typedef struct {
   const unsigned* ce_max;
   const long long* targets;
   int rows, V, H;
-  float *loss, *prob, *lse, *factor;
+  float *loss, *sum, *base, *inv_z, *factor;
   void* E;
   long long lde;
   const float* scale;
@@ -278,9 +279,9 @@ typedef struct {
 } olb_lce_finish_desc;
 // (launched so that it waits for the launch before it inside the kernel)
 int olb_lce_finish(const olb_lce_finish_desc* d, cudaStream_t stream);
-// For exponentials that were taken against the log-sum-exp: factor[r] as above (times *scale when that is not NULL; factor
-// may be NULL), and the target entries of the columns [v0, v0 + cols) in E (may be NULL): E[r, t - v0] = -prob[r] (rounded).
-int olb_lce_patch(const float* prob, const long long* targets, int rows, int V, const float* scale, float* factor, int v0,
+// For exponentials taken again against base: factor[r] as above (may be NULL), and the target entries of the columns
+// [v0, v0 + cols) in E (may be NULL): E[r, t - v0] = -sum[r] (rounded).
+int olb_lce_patch(const float* sum, const float* inv_z, const long long* targets, int rows, int V, float* factor, int v0,
                   int cols, void* E, long long lde, cudaStream_t stream);
 // row_factor[r] = factor[r] * grad[r * grad_stride] and, when xs is not NULL, xs[r, :] = bf16(row_factor[r] * x[r, :]).
 // A product launched next with `overlap` starts under this.

@@ -95,3 +95,10 @@ def test_large_logits(size, far, way):
     check(*problem(16, *LARGE[size], far=far), "mean", way)
     if way == "whole":
         check(*problem(16, *LARGE[size], far=far), "none", way)
+
+
+@pytest.mark.parametrize("size", LARGE)
+@pytest.mark.parametrize("far", [False, True])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_large_logits_computed_again(size, far, reduction):
+    check(*problem(16, *LARGE[size], far=far), reduction, "columns")
