@@ -465,6 +465,9 @@ c10::optional<at::Tensor> linear_ce(const at::Tensor& x, const at::Tensor& weigh
   TORCH_CHECK_VALUE(x.device() == weight.device() && x.device() == targets.device(), "x, weight and targets are on different devices");
   TORCH_CHECK_VALUE(max_bytes > 0, "max_workspace must be positive");
   if (x.scalar_type() != at::kBFloat16 || weight.scalar_type() != at::kBFloat16 || weight.size(1) % 8) return c10::nullopt;
+  // with or without gradients: a call without a node would lose the tangent
+  TORCH_CHECK_NOT_IMPLEMENTED(!x._fw_grad(0).defined() && !weight._fw_grad(0).defined(),
+                              "linear_cross_entropy has no forward-mode derivative for bf16 CUDA tensors");
   const at::Tensor x2 = as_rows(x), w = as_rows(weight);
   const at::Tensor flat = (targets.dim() == 1 ? targets : targets.reshape({-1})).to(at::kLong).contiguous();
   const bool grad = at::GradMode::is_enabled();

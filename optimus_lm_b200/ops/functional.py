@@ -977,7 +977,8 @@ def linear_cross_entropy(x, weight, targets, reduction="mean", max_workspace=1 <
     ``x [..., H]``, ``weight [V, H]`` (the LM head), ``targets [...]`` integers; positions whose target lies outside
     ``[0, V)`` (such as -100) are ignored: loss 0, no gradient, not counted by the mean.  ``reduction``: ``"mean"`` over
     the positions that count (NaN when there are none, as ``F.cross_entropy`` gives), ``"sum"``, or ``"none"`` for
-    losses of the targets' shape.  The loss is fp32; gradients reach ``x`` and ``weight`` (once-differentiable).
+    losses of the targets' shape.  The loss is fp32; gradients reach ``x`` and ``weight`` (once-differentiable,
+    and in reverse only: the kernel path refuses forward-mode duals).
 
     ``max_workspace`` bounds, in bytes, the exponentials of the logits held at a time (bf16, 2 V bytes for each
     position).  When those of all positions fit they are kept until the backward.  Otherwise ``"mean"`` and ``"sum"`` take

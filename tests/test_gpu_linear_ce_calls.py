@@ -1,0 +1,31 @@
+"""Calls of the cross entropy from hidden states and of the gradient clipping that the kernels have to refuse or count."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwad
+
+pytestmark = pytest.mark.gpu
+
+from optimus_lm_b200.ops import _ext, functional as OF
+
+
+def make(T, H, V, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(T, H, device="cuda", generator=g).to(torch.bfloat16)
+    w = (torch.randn(V, H, device="cuda", generator=g) * 0.05).to(torch.bfloat16)
+    return x, w, torch.randint(0, V, (T,), device="cuda", generator=g)
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("requires_grad", [True, False])
+def test_forward_mode_of_the_loss_is_refused(grad, requires_grad):
+    # no_grad does not switch forward mode off
+    x, w, t = make(40, 64, 100)
+    x.requires_grad_(requires_grad)
+    with fwad.dual_level(), torch.set_grad_enabled(grad):
+        for a, b in ((fwad.make_dual(x, torch.ones_like(x)), w), (x, fwad.make_dual(w, torch.ones_like(w)))):
+            for reduction in ("mean", "none"):
+                with pytest.raises(NotImplementedError, match="forward"):
+                    OF.linear_cross_entropy(a, b, t, reduction)
+        # types that take the plain path have the derivative
+        dual = fwad.make_dual(x.detach().float(), torch.ones(40, 64, device="cuda"))
+        assert fwad.unpack_dual(OF.linear_cross_entropy(dual, w.float(), t)).tangent is not None
