@@ -45,6 +45,8 @@ c10::optional<at::Tensor> grad_clip(const pybind11::list& items, bool inf_norm, 
     TORCH_CHECK_VALUE(g.layout() == at::kStrided, "sparse gradients are not supported");
     if (!g.is_cuda() || (g.scalar_type() != at::kBFloat16 && g.scalar_type() != at::kFloat) || g.is_conj() || g.is_neg()) return c10::nullopt;
   }
+  for (const at::Tensor& g : grads)
+    TORCH_CHECK_NOT_IMPLEMENTED(!g._fw_grad(0).defined(), "gradients that are forward-mode duals are not supported");
   c10::cuda::CUDAGuard guard(device);
   for (const at::Tensor& g : grads) {
     if (g.numel() == 0) continue;

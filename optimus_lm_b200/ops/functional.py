@@ -1173,6 +1173,7 @@ def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
     One call for any number of tensors, of any length and alignment (two launches up to 2040 tensors), bf16 and fp32 mixed;
     squares are summed in fp64 beyond 16 bytes, so that neither their number nor their size shows, and the bits are
     the same every run.  Other types and CPU tensors take the plain path.  All tensors must be on one device.
+    The norm carries no gradient; the kernel path refuses forward-mode duals.
     Reference: ``torch.nn.utils.get_total_norm`` on the parameters' gradients (dist_train.py:889-906)."""
     grads = _check_grads(grads, norm_type)
     if not grads:

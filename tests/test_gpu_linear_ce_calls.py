@@ -29,3 +29,14 @@ def test_forward_mode_of_the_loss_is_refused(grad, requires_grad):
         # types that take the plain path have the derivative
         dual = fwad.make_dual(x.detach().float(), torch.ones(40, 64, device="cuda"))
         assert fwad.unpack_dual(OF.linear_cross_entropy(dual, w.float(), t)).tangent is not None
+
+
+def test_forward_mode_of_the_clipping_is_refused():
+    g = torch.ones(100, device="cuda")
+    with fwad.dual_level():
+        dual = fwad.make_dual(g, torch.ones_like(g))
+        with pytest.raises(NotImplementedError, match="forward"):
+            OF.grad_norm([torch.zeros(3, device="cuda"), dual])
+        with pytest.raises(NotImplementedError, match="forward"):
+            OF.clip_grad_norm_([torch.zeros(3, device="cuda"), dual], 1.0)
+    assert torch.equal(g, torch.ones_like(g))
