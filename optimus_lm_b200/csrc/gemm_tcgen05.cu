@@ -463,9 +463,10 @@ __device__ __forceinline__ void epilogue_tail(const GemmParams& p, const CUtenso
 }
 
 // The split tiles of a product with EPI_ROWSCALE: sum of a tile's parts in their order, times the row's factor, rounded once
-// into C (accumulate: added to it, in fp32).  8 columns per thread.
+// into C (accumulate: added to it, in fp32).  8 columns per thread.  `part` is written by the launch under which this one
+// starts: no __restrict__, which would let its loads be moved before the wait.
 __global__ void __launch_bounds__(256)
-tail_sum_kernel(const GemmParams p, const float* __restrict__ part, int num_m, int num_n, int tile_m, int tile_n) {
+tail_sum_kernel(const GemmParams p, const float* part, int num_m, int num_n, int tile_m, int tile_n) {
   grid_dependency_wait();
   const int vecs = tile_n / 8;
   const long long a_tile = static_cast<long long>(tile_m) * tile_n;

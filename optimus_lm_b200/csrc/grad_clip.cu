@@ -212,22 +212,23 @@ grad_norm_kernel(const __grid_constant__ ClipTable<CAP> t, unsigned per_block, d
   }
 }
 
+// `partial` comes from the launch before, under which grad_scale_kernel starts: loads from the L2, which stay behind the wait.
 template <bool INF>
 __device__ __forceinline__ float clip_norm(const double* partial, int nparts, double* s) {
   if (INF) {
     unsigned top = 0;
     for (int i = threadIdx.x; i < nparts; i += CLIP_THREADS)
-      top = max(top, static_cast<unsigned>(__double_as_longlong(partial[i])));
+      top = max(top, static_cast<unsigned>(__double_as_longlong(__ldcg(partial + i))));
     return __uint_as_float(clip_block_max(top, reinterpret_cast<unsigned*>(s)));
   }
   double sum = 0.0;
-  for (int i = threadIdx.x; i < nparts; i += CLIP_THREADS) sum += partial[i];
+  for (int i = threadIdx.x; i < nparts; i += CLIP_THREADS) sum += __ldcg(partial + i);
   return static_cast<float>(sqrt(clip_block_sum(sum, s)));
 }
 
 template <bool INF>
 __global__ void __launch_bounds__(CLIP_THREADS)
-grad_norm_finish_kernel(const double* __restrict__ partial, int nparts, float* __restrict__ norm_out) {
+grad_norm_finish_kernel(const double* partial, int nparts, float* norm_out) {
   __shared__ double s[CLIP_THREADS / 32];
   const float norm = clip_norm<INF>(partial, nparts, s);
   if (threadIdx.x == 0) *norm_out = norm;
@@ -235,8 +236,8 @@ grad_norm_finish_kernel(const double* __restrict__ partial, int nparts, float* _
 
 template <int CAP, bool INF>
 __global__ void __launch_bounds__(CLIP_THREADS, 4)
-grad_scale_kernel(const __grid_constant__ ClipTable<CAP> t, unsigned per_block, const double* __restrict__ partial, int nparts,
-                  float max_norm, float eps, float* __restrict__ norm_out) {
+grad_scale_kernel(const __grid_constant__ ClipTable<CAP> t, unsigned per_block, const double* partial, int nparts,
+                  float max_norm, float eps, float* norm_out) {
   grid_dependency_wait();
   __shared__ double s[CLIP_THREADS / 32];
   const float norm = clip_norm<INF>(partial, nparts, s);
