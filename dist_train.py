@@ -340,7 +340,8 @@ def main(argv=None):
         use_activation_checkpointing=args.use_activation_checkpointing,
         activation_checkpointing_level=args.activation_checkpointing_level, use_fast_moe=args.use_fast_moe,
         use_merged_mlp_in_fast_moe=args.use_merged_mlp_in_fast_moe, force_uniform_routing=args.force_uniform_routing,
-        use_fused_ep_alltoall=not args.disable_fused_ep_alltoall)
+        use_fused_ep_alltoall=not args.disable_fused_ep_alltoall,
+        use_linear_cross_entropy=args.use_linear_cross_entropy)
     if rank == 0:
         print(config, flush=True)
     if not args.use_hf_model:
