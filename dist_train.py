@@ -141,7 +141,7 @@ def build_parser():
     p.add_argument("--router_z_loss_coef", type=float, default=0.0)
     p.add_argument("--use_linear_cross_entropy", action="store_true",
                    help="Loss and its gradients straight from the hidden states and the LM head's weight: the logits are "
-                        "never in memory (without pipeline stages and tensor parallelism; ignored otherwise)")
+                        "never in memory (without pipeline stages and tensor parallelism; otherwise without effect, with a warning)")
     p.add_argument("--opt_use_list_clipping", action="store_true",
                    help="With --opt_use_pt_optimizer: gradient norm and clipping in one call over all gradients")
     p.add_argument("--moe_capacity_factor", type=float, default=None,

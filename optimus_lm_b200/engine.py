@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import math
 import os
+import warnings
 from dataclasses import dataclass, field
 from typing import Optional
 
@@ -188,6 +189,17 @@ def get_learning_rate(step_id, train_steps, args):
     return args.min_lr + coeff * (args.lr - args.min_lr)
 
 
+def switches_without_effect(args: EngineArgs, model, pmap):
+    """What ``args`` asks for and this model, its layout or its optimizer does not do."""
+    out = []
+    if args.use_linear_cross_entropy and not (getattr(model, "use_linear_cross_entropy", False) and pmap.pipeline_parallelism == 1):
+        out.append("use_linear_cross_entropy has no effect with pipeline stages, tensor parallelism or the transformers model: "
+                   "the loss is taken over the logits")
+    if args.opt_use_list_clipping and args.optimizer != "pt":
+        out.append(f"opt_use_list_clipping has no effect on the optimizer {args.optimizer!r}: it is for \"pt\"")
+    return out
+
+
 class TrainEngine:
     def __init__(self, args: EngineArgs, pmap: Optional[ParallelDpPpEpTpMapper] = None, model=None, config=None,
                  device=None):
@@ -229,6 +241,9 @@ class TrainEngine:
             std = args.init_std if args.init_std is not None else getattr(config, "initializer_range", 0.02)
             init_weights(model, std, args.seed)
         self.config, self.model = config, model
+        if rank == 0:
+            for text in switches_without_effect(args, model, pmap):
+                warnings.warn(text)
         self.model.to(self.device)
         self.optimizer = self._build_optimizer()
         self.trainer = self._build_trainer()
