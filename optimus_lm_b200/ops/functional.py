@@ -1166,6 +1166,29 @@ def _check_grads(grads, norm_type):
     return grads
 
 
+def _check_scalable(grads):
+    """The kernel path's refusals of memory that would be scaled twice; the indices of tensors that are not dense, which are
+    scaled from copies."""
+    spans, gaps = [], []
+    for i, g in enumerate(grads):
+        if g.layout != torch.strided or g.device.type == "meta" or g.numel() == 0:
+            continue
+        span, dense = 1, True
+        for stride, size in sorted((st, n) for st, n in zip(g.stride(), g.shape) if n > 1):
+            if stride < span:
+                raise ValueError("a gradient to be scaled addresses an element more than once")
+            dense = dense and stride == span
+            span = stride * (size - 1) + span
+        if dense:
+            spans.append((g.data_ptr(), g.data_ptr() + g.numel() * g.element_size()))
+        else:
+            gaps.append(i)
+    spans.sort()
+    if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+        raise ValueError("gradients to be scaled share memory")
+    return gaps
+
+
 def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
     """Norm of all elements of the tensors ``grads`` together (Euclidean, or the largest absolute value with
     ``norm_type=inf``) as a 0-dim fp32 tensor on their device.
@@ -1207,7 +1230,9 @@ def clip_grad_norm_(grads, max_norm: float, norm_type: float = 2.0) -> torch.Ten
             return norm
     with torch.no_grad():
         norm = grad_norm(grads, norm_type)
+        copies = {i: grads[i].clone() for i in _check_scalable(grads)}
         factor = torch.clamp(max_norm / (norm + 1e-6), max=1.0)
-        for g in grads:
-            g.copy_(g.float() * factor if g.dtype != torch.float64 else g * factor)
+        for i, g in enumerate(grads):
+            old = copies.get(i, g)
+            g.copy_(old.float() * factor if g.dtype != torch.float64 else old * factor)
     return norm

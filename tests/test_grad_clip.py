@@ -52,3 +52,26 @@ def test_only_tensors(bad):
     with pytest.raises(TypeError):
         OF.clip_grad_norm_(bad, 1.0)
     assert not isinstance(bad[0], torch.Tensor) or torch.equal(bad[0], torch.ones(3))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_shared_memory_is_refused_when_scaled(dtype):
+    a = torch.ones(100, dtype=dtype)
+    m = torch.ones(6, 8, dtype=dtype)
+    for bad in ([a, a], [a[:60], a[50:]], [a, a[3:4]], [m.t(), m[2:3]], [torch.ones(1, dtype=dtype).expand(5)],
+                [torch.ones(4, dtype=dtype).as_strided((2, 3), (1, 1))]):
+        for norm_type in (2.0, math.inf):
+            with pytest.raises(ValueError, match="share memory|more than once"):
+                OF.clip_grad_norm_(bad, 0.5, norm_type)
+    assert torch.equal(a, torch.ones_like(a)) and torch.equal(m, torch.ones_like(m))
+    assert OF.grad_norm([a, a]).item() == pytest.approx(math.sqrt(200), rel=1e-6)   # reading twice is no harm
+    # neighbours, interleaved pieces, empty ones and a transposed matrix do not share
+    base = torch.ones(4, 12, dtype=dtype)
+    norm = OF.clip_grad_norm_([a[:50], a[50:], base[:, :5], base[:, 5:], a[:0], a[:0], m.t()], 0.5)
+    want = 0.5 / (norm.item() + 1e-6)
+    for t in (a, base, m):
+        assert torch.allclose(t.float(), torch.full_like(t, want).float(), rtol=2.0 ** -10)   # a step of fp16
+    # a tensor that is not dense and one that lies over it hold the same values afterwards, scaled once
+    v = torch.full((10,), 2.0, dtype=dtype)
+    norm = OF.clip_grad_norm_([v, v[::3]], 1.0)
+    assert torch.allclose(v.float(), torch.full((10,), 2 / (norm.item() + 1e-6)), rtol=2.0 ** -10)
