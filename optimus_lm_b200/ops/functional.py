@@ -1209,8 +1209,8 @@ def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
         raise TypeError("gradients must be tensors")
     if any(g.device != grads[0].device for g in grads):
         raise ValueError("the gradients are on different devices")
-    grads = [g for g in grads if g.numel()]
-    return _grad_norm_reference(grads, norm_type) if grads else torch.zeros(())
+    filled = [g for g in grads if g.numel()]
+    return _grad_norm_reference(filled, norm_type) if filled else torch.zeros((), device=grads[0].device)
 
 
 def clip_grad_norm_(grads, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:

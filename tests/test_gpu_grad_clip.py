@@ -217,3 +217,9 @@ def test_two_calls_at_once():
     for k, n in enumerate(got):
         w = wb if k % 2 else wa
         assert abs(n.item() - w) <= NORM * w
+
+
+def test_norm_of_nothing_is_on_the_device():
+    for dtype in (torch.float16, torch.bfloat16):
+        empty = [torch.zeros(0, device="cuda", dtype=dtype)]
+        assert OF.grad_norm(empty).device == OF.clip_grad_norm_(empty, 1.0).device == empty[0].device
