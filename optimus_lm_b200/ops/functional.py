@@ -1021,6 +1021,8 @@ def shifted_linear_cross_entropy(hidden, weight, labels):
     is scored against ``labels[:, s + 1]``, mean over the positions that have a target."""
     if labels.dim() != 2 or hidden.dim() != 3 or hidden.shape[:2] != labels.shape:
         raise ValueError(f"hidden [B, S, H] and labels [B, S] do not match: {tuple(hidden.shape)}, {tuple(labels.shape)}")
+    if labels.is_floating_point() or labels.is_complex() or labels.dtype == torch.bool:
+        raise ValueError(f"labels must be integers, not {labels.dtype}")   # the copy below would round them
     tgt = torch.full(labels.shape, -100, dtype=torch.long, device=labels.device)
     tgt[:, :-1] = labels[:, 1:]
     return linear_cross_entropy(hidden, weight, tgt)

@@ -53,3 +53,11 @@ def test_refusals():
         OF.shifted_linear_cross_entropy(x, w, t)
     with pytest.raises(ValueError):
         OF.shifted_linear_cross_entropy(x.view(1, 37, 16), w, t.view(37, 1))
+
+
+@pytest.mark.parametrize("bad", [torch.float32, torch.float64, torch.bool, torch.complex64])
+def test_shifted_form_takes_integer_labels(bad):
+    x, w, _ = problem(T=24)
+    with pytest.raises(ValueError, match="integers"):
+        OF.shifted_linear_cross_entropy(x.view(4, 6, 16), w, torch.ones(4, 6).to(bad))
+    assert torch.isfinite(OF.shifted_linear_cross_entropy(x.view(4, 6, 16), w, torch.ones(4, 6, dtype=torch.int32)))
