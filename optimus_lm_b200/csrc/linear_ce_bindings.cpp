@@ -6,7 +6,8 @@
 //   pieces of the batch      : for one scalar loss the incoming gradient is a common factor, so forward runs the gradient
 //                              products of each piece too (dX to bf16, dW summed in fp32) and backward scales them (one
 //                              more rounding of dX unless the gradient is a power of two); every logit is computed once, 6 T H V
-//                              operations in all.  Needs the fp32 dW within the limit as well.
+//                              operations in all.  Needs the fp32 dW within the limit as well, or where none is
+//                              wanted the exponentials of 256 rows.
 //   pieces of the vocabulary : losses per row, whose gradients the forward does not know, or a weight too large for the
 //                              fp32 dW.  Forward keeps three floats per row (what its exponentials were relative to, their
 //                              sum, 1 / Z); backward computes the same exponentials again, 8 T H V
@@ -190,7 +191,9 @@ at::Tensor linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Ten
   }
   int64_t rows_max = piece_rows(p.T, grad ? 2 * p.lde : 4 * ((p.V + 15) / 16), max_bytes);
   const bool single = rows_max >= p.T;
-  const bool store = grad && (single || (reduction != NONE && 4 * p.V * p.H <= max_bytes));
+  // pieces of the batch: the weight's fp32 gradient fits, or none is wanted and the smallest piece's exponentials fit
+  const bool in_pieces = reduction != NONE && (4 * p.V * p.H <= max_bytes || (!need_dw && 2 * p.lde * 256 <= max_bytes));
+  const bool store = grad && (single || in_pieces);
   if (grad && !store) rows_max = piece_rows(p.T, 4 * ((p.V + 15) / 16), max_bytes);
   // sums per row, of whole pieces and of a shorter last one
   const int64_t last = p.T - (p.T - 1) / rows_max * rows_max;

@@ -982,9 +982,9 @@ def linear_cross_entropy(x, weight, targets, reduction="mean", max_workspace=1 <
 
     ``max_workspace`` bounds, in bytes, the exponentials of the logits held at a time (bf16, 2 V bytes for each
     position).  When those of all positions fit they are kept until the backward.  Otherwise ``"mean"`` and ``"sum"`` take
-    the batch in pieces and compute the gradients in the forward, if an fp32 ``[V, H]`` buffer fits the bound as well; if it
-    does not, and for ``"none"``, the backward computes the logits again in pieces of the vocabulary (a third more work,
-    and an fp32 buffer of ``x``'s shape).
+    the batch in pieces and compute the gradients in the forward, if an fp32 ``[V, H]`` buffer for the weight's gradient fits
+    the bound as well (without one: the exponentials of 256 positions); if it does not, and for ``"none"``, the backward
+    computes the logits again in pieces of the vocabulary (a third more work, and an fp32 buffer of ``x``'s shape).
     (16384 tokens x 2048 against 50304, peak memory above the inputs and time: 2 GiB allowed 1.87 GiB, 7.4 to 7.9 ms; 1 GiB
     1.29 GiB, 7.8 to 8.1; 512 MiB 0.91 GiB, 8.3; 128 MiB 0.57 GiB, 10.7; over the logits 1.79 GiB, 7.5.)
 

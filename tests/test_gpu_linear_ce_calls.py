@@ -40,3 +40,21 @@ def test_forward_mode_of_the_clipping_is_refused():
         with pytest.raises(NotImplementedError, match="forward"):
             OF.clip_grad_norm_([torch.zeros(3, device="cuda"), dual], 1.0)
     assert torch.equal(g, torch.ones_like(g))
+
+
+def test_frozen_head_past_the_workspace():
+    # without a gradient of the weight there is no fp32 gradient of it that would have to fit: the forward makes the
+    # gradient of x, and the backward only scales it
+    T, H, V = 8192, 256, 20000
+    x, w, t = make(T, H, V)
+    x.requires_grad_()
+    loss = OF.linear_cross_entropy(x, w, t, max_workspace=4 * w.numel() - 1)
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    dx, = torch.autograd.grad(loss, x)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - held <= 2 * x.numel() + (1 << 16)
+    want, = torch.autograd.grad(OF.linear_cross_entropy(x, w, t, max_workspace=2 << 30), x)
+    # one more rounding to bf16
+    assert ((dx.float() - want.float()).abs() <= 2.0 ** -7 * want.float().abs() + 2.0 ** -16 * want.float().abs().max()).all()
