@@ -63,8 +63,8 @@ def use_kernels(*tensors: torch.Tensor) -> bool:
 # Kernel launches issued per binding call (see csrc/*.cu launchers).
 _LAUNCHES_PER_CALL = {
     "moe_build_index": 4, "sumsq": 2, "attn_bwd": 3,
-    "linear_ce": 5,  # the forward of one piece; its backward's three do not pass through here
-    "grad_clip": 2,
+    "linear_ce": 0,  # counts its launches, forward and backward, itself
+    "grad_clip": 2,  # up to 2040 tensors
 }
 
 
@@ -73,18 +73,27 @@ class _CountingProxy:
 
     def __init__(self, mod):
         object.__setattr__(self, "_mod", mod)
-        object.__setattr__(self, "launches", 0)
-        object.__setattr__(self, "by_name", {})
+        object.__setattr__(self, "_calls", {})
+        object.__setattr__(self, "_linear_ce0", mod.linear_ce_launches())
+
+    @property
+    def by_name(self):
+        n = self._mod.linear_ce_launches() - self._linear_ce0
+        return {**self._calls, "linear_ce": n} if n else dict(self._calls)
+
+    @property
+    def launches(self):
+        return sum(self.by_name.values())
 
     def __getattr__(self, name):
         fn = getattr(self._mod, name)
-        if not callable(fn) or name.endswith("_blocks") or name.endswith("_ints"):
+        if not callable(fn) or name.endswith(("_blocks", "_ints", "_launches")):
             return fn
         n = _LAUNCHES_PER_CALL.get(name, 1)
 
         def counted(*a, **k):
-            object.__setattr__(self, "launches", self.launches + n)
-            self.by_name[name] = self.by_name.get(name, 0) + n
+            if n:
+                self._calls[name] = self._calls.get(name, 0) + n
             return fn(*a, **k)
 
         return counted

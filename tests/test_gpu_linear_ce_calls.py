@@ -58,3 +58,34 @@ def test_frozen_head_past_the_workspace():
     want, = torch.autograd.grad(OF.linear_cross_entropy(x, w, t, max_workspace=2 << 30), x)
     # one more rounding to bf16
     assert ((dx.float() - want.float()).abs() <= 2.0 ** -7 * want.float().abs() + 2.0 ** -16 * want.float().abs().max()).all()
+
+
+# sizes whose products split their last wave and do not, every way to hold the exponentials, without gradients
+COUNTED = [("mean", 300, 1000, 3000, {}, "xw"), ("sum", 512, 256, 1024, {}, "xw"), ("none", 600, 64, 500, {"max_workspace": 1}, "xw"),
+           ("mean", 600, 64, 500, {"max_workspace": 4 * 64 * 500}, "xw"), ("mean", 600, 64, 500, {"max_workspace": 4 * 64 * 500}, "x"),
+           ("none", 40, 64, 500, {}, "w"), ("none", 40, 64, 500, {}, "")]
+
+
+@pytest.mark.parametrize("reduction,T,H,V,kw,need", COUNTED)
+def test_launches_are_counted(reduction, T, H, V, kw, need):
+    x, w, t = make(T, H, V)
+    leaves = [v.requires_grad_() for v, n in ((x, "x"), (w, "w")) if n in need]
+
+    def call():
+        loss = OF.linear_cross_entropy(x, w, t, reduction, **kw)
+        if leaves:
+            torch.autograd.grad(loss, leaves, torch.ones_like(loss))
+        torch.cuda.synchronize()
+
+    call()
+    proxy = _ext.enable_launch_counting()
+    try:
+        before = proxy.launches, proxy.by_name.get("linear_ce", 0)
+        with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA, torch.profiler.ProfilerActivity.CPU]) as prof:
+            call()
+        counted = proxy.launches - before[0]
+        assert proxy.by_name["linear_ce"] - before[1] == counted
+    finally:
+        _ext._C = proxy._mod
+    seen = [e.name for e in prof.events() if e.device_type == torch.autograd.DeviceType.CUDA and "olb::" in e.name]
+    assert counted == len(seen) > 0, (counted, seen)
