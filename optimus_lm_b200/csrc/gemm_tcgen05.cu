@@ -162,6 +162,8 @@ constexpr int NUM_THREADS_STAGED = NUM_THREADS + 32 * STAGER_WARPS;
 // Epilogue warps of a CTA and threads of a launch (EPI_CE: sixteen, see epilogue_ce).
 __host__ __device__ constexpr int epilogue_warps(int epi) { return epi == EPI_CE ? 16 : 4; }
 __host__ __device__ constexpr int num_threads(bool peer, int epi) { return peer ? NUM_THREADS_STAGED : 64 + 32 * epilogue_warps(epi); }
+// Launches that may start under the one before them (GemmParams::overlap).
+__host__ __device__ constexpr bool may_overlap(bool peer, int epi) { return !peer && (epi == EPI_CE || epi == EPI_ROWSCALE); }
 
 // Epilogue staging: each of the four epilogue warps owns two buffers of 32 rows x 128 bytes (what one tensor-map
 // store of its rows takes), laid out with the 128-byte swizzle the store expects.
@@ -923,7 +925,9 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
   constexpr uint32_t TMEM_COLS = (2 * BLOCK_N < 32) ? 32 : 2 * BLOCK_N;
   static_assert(EPI != EPI_SWIGLU || BLOCK_N == 256, "the SwiGLU epilogue pairs 128 gate with 128 up columns");
 
-  if (p.overlap) grid_launch_dependents();
+  if constexpr (may_overlap(PEER, EPI)) {
+    if (p.overlap) grid_launch_dependents();
+  }
   if constexpr (EPI == EPI_CE) {
     if (p.ce_repair) {
       if (p.overlap) grid_dependency_wait();  // every thread: this launch ends after the one before it
@@ -1118,7 +1122,9 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
     }
   } else if (warp < 2 + epilogue_warps(EPI)) {
     // ------------------------------------------------------------ epilogue (warps 2..5)
-    if (p.overlap) grid_dependency_wait();
+    if constexpr (may_overlap(PEER, EPI)) {
+      if (p.overlap) grid_dependency_wait();
+    }
     const int lane_group = warp & 3;  // TMEM lanes [32*lane_group, +32) belong to this warp
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -1247,7 +1253,9 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
   constexpr int BLOCK_N = 256;
   constexpr uint32_t TMEM_COLS = 512;
 
-  if (p.overlap) grid_launch_dependents();
+  if constexpr (may_overlap(PEER, EPI)) {
+    if (p.overlap) grid_launch_dependents();
+  }
   if constexpr (EPI == EPI_CE) {
     if (p.ce_repair) {
       if (p.overlap) grid_dependency_wait();  // every thread: this launch ends after the one before it
@@ -1437,7 +1445,9 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
     }
   } else if (warp < 2 + epilogue_warps(EPI)) {
     // ------------------------------------------------------------ epilogue (warps 2..5 of both CTAs, own 128 rows)
-    if (p.overlap) grid_dependency_wait();
+    if constexpr (may_overlap(PEER, EPI)) {
+      if (p.overlap) grid_dependency_wait();
+    }
     const int lane_group = warp & 3;
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -1652,7 +1662,7 @@ static int launch(const TensorMaps& tm, const PeerArg<PEER>& peers, const GemmPa
   if (EPI == EPI_ROWSCALE && p.tail_splits > 1) tiles = p.tail_from + (tiles - p.tail_from) * p.tail_splits;
   int grid = static_cast<int>(tiles < num_sms ? tiles : num_sms);
   if (grid <= 0) return 0;
-  if constexpr (!PEER && (EPI == EPI_CE || EPI == EPI_PLAIN || EPI == EPI_ROWSCALE)) {
+  if constexpr (may_overlap(PEER, EPI)) {
     if (p.overlap)
       return launch_overlapped(gemm_bf16_kernel<BLOCK_N, PEER, EPI>, grid, num_threads(PEER, EPI), L::TOTAL, stream, tm, peers, p);
   }
@@ -1682,7 +1692,7 @@ static int launch_pair(const TensorMaps& tm, const PeerArg<PEER>& peers, const G
   const int max_pairs = num_sms / 2;
   const int pairs = static_cast<int>(tiles < max_pairs ? tiles : max_pairs);
   if (pairs <= 0) return 0;
-  if constexpr (!PEER && (EPI == EPI_CE || EPI == EPI_PLAIN || EPI == EPI_ROWSCALE)) {
+  if constexpr (may_overlap(PEER, EPI)) {
     if (p.overlap)
       return launch_overlapped(gemm_bf16_pair_kernel<PEER, EPI>, 2 * pairs, num_threads(PEER, EPI), L::TOTAL, stream, tm, peers, p);
   }
@@ -1844,7 +1854,9 @@ extern "C" long long olb_gemm_tail_floats(const olb_gemm_desc* d) {
 extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   using namespace olb;
   if (d->M <= 0 || d->N <= 0) return 0;
-  if (d->overlap && (d->mode != OLB_GEMM_DENSE || d->n_peers || d->accumulate || d->c_reduce)) return -23;
+  if (d->overlap && ((d->epilogue != OLB_EPI_CE && d->epilogue != OLB_EPI_ROWSCALE) || d->mode != OLB_GEMM_DENSE || d->n_peers ||
+                     d->accumulate || d->c_reduce))
+    return -23;
   if ((d->lda % 8) || (d->ldb % 8) || (d->ldc % 8) || (d->N % 8 && d->epilogue != OLB_EPI_CE) || (reinterpret_cast<uintptr_t>(d->A) & 15) ||
       (reinterpret_cast<uintptr_t>(d->B) & 15) || (reinterpret_cast<uintptr_t>(d->C) & 15))
     return -10;

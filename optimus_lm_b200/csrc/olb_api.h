@@ -115,7 +115,7 @@ typedef struct {
   long long ce_part_ld;
   int* ce_flags;
   int ce_repair;
-  // DENSE, C written and not read: start while the launch before this one on the stream is still running, if that allows
+  // OLB_EPI_CE or OLB_EPI_ROWSCALE, C written and not read: start while the launch before this one on the stream is still running, if that allows
   // it; only the epilogue (row_scale, ce_*, the stores to C) waits for its end.  For a launch whose A and B do not come from
   // the one before it.  The launch after this one may start early in turn.
   int overlap;
