@@ -141,3 +141,116 @@ def test_replay_catches_a_barrier_that_is_one_arrival_short():
         except AssertionError:
             failures += 1
     assert failures > 0
+
+
+class CeBarrier(TxBarrier):
+    """The barrier with the arrivals by warp, so that none may arrive twice in a phase."""
+
+    def __init__(self, count):
+        super().__init__(count)
+        self.who = set()
+
+    def arrive_from(self, warp):
+        assert warp not in self.who, "a warp arrived twice in one phase"
+        self.who.add(warp)
+        done = self.completions
+        self.arrive()
+        if self.completions != done:
+            self.who.clear()
+
+
+def ce_roles(tiles, k_blocks, STAGES, ctas, live_warps, flagged, warps=16, arrivals=None, early=False):
+    """The cross-entropy epilogue: sixteen epilogue warps in each of one or two CTAs.  A warp reads its columns of the
+    accumulator (tcgen05.ld), waits for them (tcgen05.wait::ld), fences and arrives; the arrive is relaxed, so nothing but that
+    order keeps the accumulator whole.  A warp whose columns lie past the tile or whose rows lie past the batch reads nothing
+    and arrives all the same (live_warps: those that read).  A repairing launch passes over the tiles that are not `flagged`
+    in every role alike.  early: the mistake of arriving before the loads have been waited for."""
+    HALF = 32768
+    full = [TxBarrier(1) for _ in range(STAGES)]
+    empty = [[TxBarrier(1) for _ in range(STAGES)] for _ in range(ctas)]
+    acc_full = [[TxBarrier(1) for _ in range(2)] for _ in range(ctas)]
+    acc_empty = [CeBarrier(ctas * warps if arrivals is None else arrivals) for _ in range(2)]
+    holds = [[None] * STAGES for _ in range(ctas)]
+    consumed, in_flight = set(), [0, 0]
+    acc_tile = [None, None]
+    todo = [t for t in range(tiles) if t in flagged]
+
+    def producer(rank):
+        i = 0
+        for _ in todo:
+            for _kb in range(k_blocks):
+                s = i % STAGES
+                if i >= STAGES:
+                    yield (empty[rank][s], i // STAGES - 1)
+                    assert holds[rank][s] in consumed, "stage refilled before the products that read it"
+                if rank == 0:
+                    full[s].arrive(expect=ctas * HALF)
+                    yield None
+                holds[rank][s] = i
+                full[s].complete_tx(HALF)
+                i += 1
+                yield None
+
+    def issuer():
+        i = 0
+        for n, t in enumerate(todo):
+            a = n & 1
+            if n >= 2:
+                yield (acc_empty[a], n // 2 - 1)
+            assert in_flight[a] == 0, "accumulator overwritten under a warp's loads"
+            acc_tile[a] = t
+            for _kb in range(k_blocks):
+                s = i % STAGES
+                yield (full[s], i // STAGES)
+                assert all(h[s] == i for h in holds), "products issued on a stage that is not complete"
+                consumed.add(i)
+                for e in empty:
+                    e[s].arrive()
+                i += 1
+                yield None
+            for f in acc_full:
+                f[a].arrive()
+            yield None
+
+    def epilogue(rank, warp):
+        for n, t in enumerate(todo):
+            a = n & 1
+            yield (acc_full[rank][a], n // 2)
+            if warp in live_warps:
+                for _turn in range(2):      # the exponentials; the maximum of a row that is far above its target
+                    assert acc_tile[a] == t, "columns of another tile"
+                    in_flight[a] += 1
+                    yield None
+                    if early and _turn == 1:
+                        acc_empty[a].arrive_from((rank, warp))
+                        yield None
+                    assert acc_tile[a] == t, "columns of another tile"
+                    in_flight[a] -= 1
+            if not (early and warp in live_warps):
+                acc_empty[a].arrive_from((rank, warp))
+            yield None
+
+    roles = [producer(r) for r in range(ctas)] + [issuer()] + [epilogue(r, w) for r in range(ctas) for w in range(warps)]
+    return roles, consumed, todo
+
+
+@pytest.mark.parametrize("tiles,k_blocks", [(1, 1), (2, 3), (9, 2), (5, 13)])
+@pytest.mark.parametrize("ctas,STAGES", [(1, 3), (1, 4), (2, 2), (2, 6)])
+@pytest.mark.parametrize("live_warps", [range(16), range(4), range(0, 16, 4)])
+def test_cross_entropy_epilogue_protocol(tiles, k_blocks, ctas, STAGES, live_warps):
+    for seed in range(5):
+        for flagged in (range(tiles), range(0, tiles, 3), ()):
+            roles, consumed, todo = ce_roles(tiles, k_blocks, STAGES, ctas, live_warps, flagged)
+            run(roles, seed)
+            assert len(consumed) == len(todo) * k_blocks
+
+
+@pytest.mark.parametrize("mistake", [dict(arrivals=28), dict(early=True)])
+def test_cross_entropy_replay_catches(mistake):
+    failures = 0
+    for seed in range(10):
+        try:
+            run(ce_roles(60, 1, 4, 2, range(16), range(60), **mistake)[0], seed)
+        except AssertionError:
+            failures += 1
+    assert failures > 0
