@@ -102,3 +102,24 @@ def test_large_logits(size, far, way):
 @pytest.mark.parametrize("reduction", ["mean", "none"])
 def test_large_logits_computed_again(size, far, reduction):
     check(*problem(16, *LARGE[size], far=far), reduction, "columns")
+
+
+@pytest.mark.parametrize("H", [64, 2048, 7168])
+def test_mean_loss_of_random_hidden_states(H):
+    # The signed error of the mean, which the rounding of single logits leaves and a factor on all of them does not.  A step of
+    # 16 terms truncates the running sum s by less than a step of fp32 of it, the 16 products' own truncations have random
+    # signs (another step): |mean error| <= 2 2^-23 mean_r sum_v p_v sum_k |s_k|, and 2^-20 of the loss for exp, sums and log.
+    T, V = 64, 500
+    g = torch.Generator(device="cuda").manual_seed(H)
+    x = torch.randn(T, H, device="cuda", generator=g).to(torch.bfloat16)
+    w = (torch.randn(V, H, device="cuda", generator=g) * (3.0 / H ** 0.5)).to(torch.bfloat16)
+    t = torch.randint(0, V, (T,), device="cuda", generator=g)
+    steps = torch.einsum("tkh,vkh->tvk", x.double().view(T, H // 16, 16), w.double().view(V, H // 16, 16)).cumsum(2)
+    l = steps[..., -1]
+    p = torch.softmax(l, 1)
+    want = (torch.logsumexp(l, 1) - l.gather(1, t[:, None])[:, 0])
+    bound = 2 * U32 * (p * steps.abs().sum(2)).sum(1).mean() + 2.0 ** -20 * want.mean()
+    with torch.no_grad():
+        off = (OF.linear_cross_entropy(x, w, t, "none").double() - want).mean().abs()
+        off_mean = (OF.linear_cross_entropy(x, w, t).double() - want.mean()).abs()
+    assert off <= bound and off_mean <= bound, (off.item(), off_mean.item(), bound.item())
