@@ -92,7 +92,7 @@ struct GemmParams {
   // EPI_CE: see epilogue_ce.
   const long long* ce_targets;
   int ce_v0, ce_v_total;       // B's rows are [ce_v0, ce_v0 + N) of a vocabulary of ce_v_total
-  const float* ce_ref;
+  const float *ce_ref, *ce_grow;
   unsigned* ce_max;
   float* ce_part;
   long long ce_part_ld;
@@ -645,10 +645,11 @@ __device__ __forceinline__ bool ce_skip_tile(const GemmParams& p, const TileInfo
 // rows without a target give zeros.  A row whose sum shows a logit more than CE_RANGE above the reference has its
 // largest logit recorded in ce_max and its row block flagged; a second launch (ce_repair) computes those blocks again
 // against the recorded maxima.
-// The logits are what the tensor cores sum.  These truncate as they add, towards zero: sums of H terms of random sign come
-// out smaller by 1.4e-8 of themselves for every 16 terms (measured: 4.0e-7 at H = 512, 1.8e-6 at 2048, 6.9e-6 at 7168), sums
-// of one sign by up to 6e-8, sums without anything to round not at all.  No factor gives that back for all of them (the
-// first one's, 1 + 1.4e-8 H / 16, is an error of 6e-6 for a logit that comes from a few of 7168 channels): none is applied.
+// The tensor cores truncate as they add, towards zero: against the exact sum a logit of H terms of random sign comes out
+// smaller by 1.4e-8 of itself for every 16 of them (measured: 4.0e-7 at H = 512, 1.8e-6 at 2048, 6.9e-6 at 7168), which is the
+// running sum's share and the mean loss's bias.  ce_grow[row] (made with the reference, lce_grow) gives that share back: l +
+// l ce_grow.  Channels that are zero add nothing to truncate and are not counted.  It is a mean: sums of one sign lose up to 6e-8
+// and get part of it back, sums of many terms that all fit 24 bits lose nothing and come out larger by it.
 // CE_RANGE: sums of 2^31 terms of e^40 = 2.4e17 stay below 1e27, far inside fp32 and bf16, and so does their inverse.
 //
 // Sixteen warps per CTA work on a tile: each four take a quarter of its columns (a warp's dependent instructions leave
@@ -674,6 +675,8 @@ __device__ __forceinline__ void epilogue_ce(const GemmParams& p, uint32_t stage,
   constexpr float LOG2E = 1.4426950408889634f;
   const float ref = live ? ce_row_ref(p, row) : 0.f;
   const float2 neg_ref = make_float2(-ref, -ref);
+  const float gain = live ? p.ce_grow[row] : 1e-30f;
+  const float2 grow = make_float2(gain, gain);
   const float2 log2e = make_float2(LOG2E, LOG2E);
   const uint32_t cols = taddr + part * COLS;
   float2 sum = make_float2(0.f, 0.f);
@@ -699,7 +702,8 @@ __device__ __forceinline__ void epilogue_ce(const GemmParams& p, uint32_t stage,
     }
 #pragma unroll
     for (int i = 0; i < CHUNK / 2; ++i) {
-      const float2 d = mul2(add2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), neg_ref), log2e);
+      const float2 l = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+      const float2 d = mul2(fma2(l, grow, add2(l, neg_ref)), log2e);
       r[2 * i] = __float_as_uint(ex2_approx(d.x));
       r[2 * i + 1] = __float_as_uint(ex2_approx(d.y));
     }
@@ -1884,7 +1888,7 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
     // C = exponentials [M, N] (row stride ldc); dense, both operands K-major
     if (d->a_mn_major || d->b_mn_major || d->accumulate || d->out_fp32 || d->mode != OLB_GEMM_DENSE || d->n_peers ||
         d->k_split || d->ce_v0 < 0 || (d->ce_v_total && d->ce_v_total < d->ce_v0 + d->N) ||
-        (d->ce_v_total == 0 && d->ce_v0) || d->ce_targets == nullptr || d->ce_ref == nullptr ||
+        (d->ce_v_total == 0 && d->ce_v0) || d->ce_targets == nullptr || d->ce_ref == nullptr || d->ce_grow == nullptr ||
         (d->ce_repair && (d->ce_flags == nullptr || d->ce_max == nullptr)) || (d->ce_flags != nullptr && d->ce_max == nullptr) ||
         (d->ce_part != nullptr && d->ce_part_ld < d->M))
       return -18;
@@ -2004,6 +2008,7 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
   p.ce_v0 = d->ce_v0;
   p.ce_v_total = d->ce_v_total ? d->ce_v_total : d->N;
   p.ce_ref = d->ce_ref;
+  p.ce_grow = d->ce_grow;
   p.ce_max = d->ce_max;
   p.ce_part = d->ce_part;
   p.ce_part_ld = d->ce_part_ld;

@@ -48,13 +48,17 @@ __device__ __forceinline__ void lce_count(const long long* __restrict__ targets,
   }
 }
 
+// What the tensor cores' running sum loses on average of a logit whose x has `vecs` vectors of 8 channels that are not all
+// zero, relative to it (see epilogue_ce); the first 16 channels are added to nothing.  Never 0, so that -inf stays -inf.
+__device__ __forceinline__ float lce_grow(int vecs) { return fmaxf(0.7e-8f * (vecs - 2), 1e-30f); }
+
 // ref[r] = x_r . w_t: one warp per row, or the block's eight for one row when there are few (a single row of 4096:
 // 6.7 us with one warp).  The last block counts the targets (`count` set).
 template <bool FEW>
 __global__ void __launch_bounds__(LCE_THREADS)
 lce_prep_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, const __nv_bfloat16* __restrict__ w, long long ldw,
                 const long long* __restrict__ targets, int rows, int H, int V, float* __restrict__ ref,
-                unsigned* __restrict__ ce_max, int* __restrict__ ce_flags, unsigned* __restrict__ ticket,
+                float* __restrict__ grow, unsigned* __restrict__ ce_max, int* __restrict__ ce_flags, unsigned* __restrict__ ticket,
                 const long long* __restrict__ all_targets, long long n_all, float* __restrict__ count) {
   // the product may start: nothing of it but its epilogue needs what this kernel writes
   grid_launch_dependents();
@@ -63,6 +67,7 @@ lce_prep_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, const __nv_b
     return;
   }
   __shared__ float s_part[LCE_WARPS];
+  __shared__ int s_used[LCE_WARPS];
   const int warp = threadIdx.x >> 5, lane = FEW ? threadIdx.x : threadIdx.x & 31;
   constexpr int LANES = FEW ? LCE_THREADS : 32;
   const int row = FEW ? blockIdx.x : blockIdx.x * LCE_WARPS + warp;
@@ -73,6 +78,7 @@ lce_prep_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, const __nv_b
   if (row >= rows) return;
   const long long t = targets[row];
   float acc = 0.f;
+  int used = 0;
   if (t >= 0 && t < V) {
     const uint4* a = reinterpret_cast<const uint4*>(x + row * ldx);
     const uint4* b = reinterpret_cast<const uint4*>(w + t * ldw);
@@ -81,22 +87,32 @@ lce_prep_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, const __nv_b
 #pragma unroll 4
     for (int i = lane; i < vecs; i += LANES) {
       const uint4 u = a[i], v = b[i];
+      used += ((u.x | u.y | u.z | u.w) & 0x7fff7fffu) != 0;
       s0 = fma2(unpack_bf16(u.x), unpack_bf16(v.x), s0);
       s1 = fma2(unpack_bf16(u.y), unpack_bf16(v.y), s1);
       s0 = fma2(unpack_bf16(u.z), unpack_bf16(v.z), s0);
       s1 = fma2(unpack_bf16(u.w), unpack_bf16(v.w), s1);
     }
     acc = warp_sum((s0.x + s0.y) + (s1.x + s1.y));
+    used = __reduce_add_sync(0xffffffffu, used);
   }
   if (FEW) {
-    if ((threadIdx.x & 31) == 0) s_part[warp] = acc;
+    if ((threadIdx.x & 31) == 0) {
+      s_part[warp] = acc;
+      s_used[warp] = used;
+    }
     __syncthreads();
     acc = 0.f;
+    used = 0;
 #pragma unroll
-    for (int i = 0; i < LCE_WARPS; ++i) acc += s_part[i];
+    for (int i = 0; i < LCE_WARPS; ++i) {
+      acc += s_part[i];
+      used += s_used[i];
+    }
   }
   if (lane == 0) {
     ref[row] = acc;
+    grow[row] = lce_grow(used);
     ce_max[row] = 0;
     if (row % 128 == 0) ce_flags[1 + row / 128] = 0;
   }
@@ -313,7 +329,7 @@ static int launched() { return cudaGetLastError() == cudaSuccess ? 0 : -2; }
 using namespace olb;
 
 extern "C" int olb_lce_prep(const void* x, long long ldx, const void* w, long long ldw, const long long* targets, int rows,
-                            int H, int V, float* ref, unsigned* ce_max, int* ce_flags, unsigned* ticket,
+                            int H, int V, float* ref, float* grow, unsigned* ce_max, int* ce_flags, unsigned* ticket,
                             const long long* all_targets, long long n_all, float* count, cudaStream_t stream) {
   if (H % 8 || ldx % 8 || ldw % 8 || misaligned(x) || misaligned(w) || n_all >= (1ll << 31)) return -1;
   if (rows <= 0) return 0;
@@ -321,11 +337,11 @@ extern "C" int olb_lce_prep(const void* x, long long ldx, const void* w, long lo
   const auto* wb = static_cast<const __nv_bfloat16*>(w);
   const int extra = count != nullptr ? 1 : 0;
   if (rows <= 148 * 8)
-    lce_prep_kernel<true><<<rows + extra, LCE_THREADS, 0, stream>>>(xb, ldx, wb, ldw, targets, rows, H, V, ref, ce_max,
+    lce_prep_kernel<true><<<rows + extra, LCE_THREADS, 0, stream>>>(xb, ldx, wb, ldw, targets, rows, H, V, ref, grow, ce_max,
                                                                     ce_flags, ticket, all_targets, n_all, count);
   else
     lce_prep_kernel<false><<<(rows + LCE_WARPS - 1) / LCE_WARPS + extra, LCE_THREADS, 0, stream>>>(
-        xb, ldx, wb, ldw, targets, rows, H, V, ref, ce_max, ce_flags, ticket, all_targets, n_all, count);
+        xb, ldx, wb, ldw, targets, rows, H, V, ref, grow, ce_max, ce_flags, ticket, all_targets, n_all, count);
   return launched();
 }
 

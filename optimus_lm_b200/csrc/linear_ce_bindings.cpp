@@ -9,8 +9,8 @@
 //                              operations in all.  Needs the fp32 dW within the limit as well, or where none is
 //                              wanted the exponentials of 256 rows.
 //   pieces of the vocabulary : losses per row, whose gradients the forward does not know, or a weight too large for the
-//                              fp32 dW.  Forward keeps three floats per row (what its exponentials were relative to, their
-//                              sum, 1 / Z); backward computes the same exponentials again, 8 T H V
+//                              fp32 dW.  Forward keeps four floats per row (what its exponentials were relative to, ce_grow,
+//                              their sum, 1 / Z); backward computes the same exponentials again, 8 T H V
 //                              operations in all, dX summed in fp32 over the pieces, dW's rows finished piece by piece.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -36,7 +36,7 @@ inline void check(int rc, const char* what, int n = 1) {
 enum { MEAN = 0, SUM = 1, NONE = 2 };
 
 // What forward leaves to backward: the exponentials and row factors; or the gradients of a scalar loss (dx, and dw in
-// fp32; undefined where not wanted); or the rows' sum, 1 / Z and reference, as [3, T].
+// fp32; undefined where not wanted); or the rows' sum, 1 / Z, reference and ce_grow, as [4, T].
 enum { PIECE = 0, SCALE = 1, AGAIN = 2 };
 struct Kept {
   int64_t kind = PIECE;
@@ -90,7 +90,7 @@ void rowscale_product(const Problem& p, olb_gemm_desc& d, const char* what) {
 
 // e = exp(l - ref) of some rows and columns [v0, v0 + cols) of the vocabulary (and the sums of their tiles), then of the
 // row blocks that need another reference.
-void product(const Problem& p, int64_t r0, int64_t rows, int64_t v0, int64_t cols, const float* ref, unsigned* top, int* flags,
+void product(const Problem& p, int64_t r0, int64_t rows, int64_t v0, int64_t cols, const float* ref, const float* grow, unsigned* top, int* flags,
              float* part, int64_t part_ld, void* E, int64_t lde, bool behind_prep) {
   olb_gemm_desc d{};
   d.A = row_ptr(p.x, r0);
@@ -110,6 +110,7 @@ void product(const Problem& p, int64_t r0, int64_t rows, int64_t v0, int64_t col
   d.status = p.status;
   d.ce_targets = ptr_i64(p.targets, r0);
   d.ce_ref = ref;
+  d.ce_grow = grow;
   d.ce_max = top;
   d.ce_flags = flags;
   d.ce_part = part;
@@ -208,12 +209,13 @@ at::Tensor linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Ten
                                        olb_gemm_ce_slices(static_cast<int>(last), static_cast<int>(p.V)));
 
   at::Tensor out = reduction == NONE ? at::empty({p.T}, f32) : at::empty({}, f32);
-  // small per-row and per-launch words: (losses,) ref, top, flags, ticket, count, 1 / count
+  // small per-row and per-launch words: (losses,) ref, grow, top, flags, ticket, count, 1 / count
   const int64_t losses = reduction == NONE ? 0 : p.T;
-  at::Tensor words = at::empty({losses + 2 * rows_max + (rows_max + 127) / 128 + 1 + 3}, f32);
+  at::Tensor words = at::empty({losses + 3 * rows_max + (rows_max + 127) / 128 + 1 + 3}, f32);
   float* loss_rows = reduction == NONE ? out.data_ptr<float>() : words.data_ptr<float>();
   float* ref = words.data_ptr<float>() + losses;
-  unsigned* top = reinterpret_cast<unsigned*>(ref + rows_max);
+  float* grow = ref + rows_max;
+  unsigned* top = reinterpret_cast<unsigned*>(grow + rows_max);
   int* flags = reinterpret_cast<int*>(top + rows_max);
   unsigned* ticket = reinterpret_cast<unsigned*>(flags + (rows_max + 127) / 128 + 1);
   float* count = reinterpret_cast<float*>(ticket + 1);
@@ -231,14 +233,15 @@ at::Tensor linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Ten
       xs = at::empty({rows_max, p.H}, x.options());
     }
   }
-  if (grad && !store) stats = at::empty({3, p.T}, f32);
+  if (grad && !store) stats = at::empty({4, p.T}, f32);
   for (int64_t r0 = 0; r0 < p.T; r0 += rows_max) {
     const int64_t rows = std::min(rows_max, p.T - r0);
+    if (stats.defined()) grow = stats.data_ptr<float>() + 3 * p.T + r0;
     check(olb_lce_prep(row_ptr(x, r0), x.stride(0), w.data_ptr(), w.stride(0), ptr_i64(p.targets, r0), static_cast<int>(rows),
-                       static_cast<int>(p.H), static_cast<int>(p.V), ref, top, flags, ticket, ptr_i64(p.targets, 0), p.T,
+                       static_cast<int>(p.H), static_cast<int>(p.V), ref, grow, top, flags, ticket, ptr_i64(p.targets, 0), p.T,
                        reduction == MEAN && r0 == 0 ? count : nullptr, p.stream),
           "olb_lce_prep");
-    product(p, r0, rows, 0, p.V, ref, top, flags, part.data_ptr<float>(), rows_max, store ? E.data_ptr() : nullptr, p.lde, true);
+    product(p, r0, rows, 0, p.V, ref, grow, top, flags, part.data_ptr<float>(), rows_max, store ? E.data_ptr() : nullptr, p.lde, true);
     olb_lce_finish_desc f{};
     f.part = part.data_ptr<float>();
     f.part_ld = rows_max;
@@ -341,8 +344,8 @@ std::vector<at::Tensor> linear_ce_bwd_again(const at::Tensor& x, const at::Tenso
   c10::cuda::CUDAGuard guard(x.device());
   const Problem p = make_problem(x, w, targets, status);
   TORCH_CHECK(grad.scalar_type() == at::kFloat && grad.device() == x.device() && grad.is_contiguous() &&
-              (grad.dim() == 0 || grad.numel() == p.T) && stats.is_contiguous() && stats.numel() == 3 * p.T);
-  const float *sum = stats.data_ptr<float>(), *inv_z = sum + p.T, *base = inv_z + p.T;
+              (grad.dim() == 0 || grad.numel() == p.T) && stats.is_contiguous() && stats.numel() == 4 * p.T);
+  const float *sum = stats.data_ptr<float>(), *inv_z = sum + p.T, *base = inv_z + p.T, *grow = base + p.T;
   const auto f32 = x.options().dtype(at::kFloat);
   const int64_t most = std::max<int64_t>(256, max_bytes / (2 * p.T) / 256 * 256);
   const int64_t pieces = (p.V + most - 1) / most;
@@ -363,7 +366,7 @@ std::vector<at::Tensor> linear_ce_bwd_again(const at::Tensor& x, const at::Tenso
         "olb_lce_scale_rows");
   for (int64_t v0 = 0; v0 < p.V; v0 += cols_max) {
     const int64_t cols = std::min(cols_max, p.V - v0);
-    product(p, 0, p.T, v0, cols, base, nullptr, nullptr, nullptr, 0, E.data_ptr(), lde, false);
+    product(p, 0, p.T, v0, cols, base, grow, nullptr, nullptr, nullptr, 0, E.data_ptr(), lde, false);
     check(olb_lce_patch(sum, inv_z, ptr_i64(p.targets, 0), T, V, nullptr, static_cast<int>(v0), static_cast<int>(cols), E.data_ptr(),
                         lde, p.stream),
           "olb_lce_patch");

@@ -101,7 +101,7 @@ typedef struct {
   float* tail_part;
   // Cross-entropy product (epilogue == OLB_EPI_CE; DENSE, K-major operands): A = hidden states, B = the head's weight
   // [N, K] with any number of rows N.  Row r has its target in ce_targets[r] (outside [0, N): no target) and a reference
-  // ce_ref[r]; with l the logits, C (may be NULL) receives exp(l - ref) as bf16, zeros for rows without a target and up to
+  // ce_ref[r]; with l the logits, enlarged by ce_grow[r] (> 0) of themselves, C (may be NULL) receives exp(l - ref) as bf16, zeros for rows without a target and up to
   // the next multiple of 32 columns, and ce_part[i * ce_part_ld + r] (may be NULL) the sum of exp(l - ref) over the i-th
   // of olb_gemm_ce_slices(M, N) slices of the columns without the target's column.  ce_flags (may be NULL; 1 + ceil(M / 128) ints and ce_max M words, all
   // zero): a row whose largest logit exceeds its reference by more than 40 has it recorded in ce_max and its block of
@@ -109,7 +109,7 @@ typedef struct {
   // With ce_v_total, B holds rows [ce_v0, ce_v0 + N) of a vocabulary of that many and targets count in the whole of it.
   const long long* ce_targets;
   int ce_v0, ce_v_total;
-  const float* ce_ref;
+  const float *ce_ref, *ce_grow;
   unsigned* ce_max;
   float* ce_part;
   long long ce_part_ld;
@@ -244,11 +244,11 @@ int olb_ce_partial_bwd(const void* logits, long long ldl, const long long* label
 
 // ---------------------------------------------------------------- cross entropy from hidden states (linear_ce.cu)
 // The passes around the OLB_EPI_CE product; `rows` is one piece of the batch (see linear_ce.cu for the formulas).
-// ref[r] = x_r . w_t (fp32) for rows with a target t in [0, V), else 0; zeroes ce_max [rows], ce_flags
+// ref[r] = x_r . w_t (fp32) for rows with a target t in [0, V), else 0; grow[r]: the product's ce_grow; zeroes ce_max [rows], ce_flags
 // [1 + ceil(rows / 128)] and *ticket.  With count: count[0] = number of all_targets [n_all] in [0, V) (as fp32, rounded
 // above 2^24), count[1] = 1 / that (0 when there are none).  A product launched next with `overlap` starts under this.
 int olb_lce_prep(const void* x, long long ldx, const void* w, long long ldw, const long long* targets, int rows, int H,
-                 int V, float* ref, unsigned* ce_max, int* ce_flags, unsigned* ticket, const long long* all_targets,
+                 int V, float* ref, float* grow, unsigned* ce_max, int* ce_flags, unsigned* ticket, const long long* all_targets,
                  long long n_all, float* count, cudaStream_t stream);
 // Sums ce_part over its `ntiles` tiles and writes per row loss[r] (0 without a target) and, when they are not NULL,
 // sum[r] (of the exponentials without the target's), base[r] (what they are relative to) and inv_z[r] = 1 / (sum and the
