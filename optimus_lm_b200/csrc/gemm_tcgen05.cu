@@ -637,8 +637,8 @@ __device__ __forceinline__ bool ce_skip_tile(const GemmParams& p, const TileInfo
 
 // Epilogue of one 128-row tile of the cross-entropy product: the accumulator holds the logits l of the row against
 // vocabulary columns [ti.n0, ti.n0 + BLOCK_N).  With the row's reference m (its target's logit, or a maximum that
-// is known already) it writes e = exp(l - m) as bf16 to C (ce_store) and the row's sum of e over half a tile without
-// the target's column to ce_part[half tile][row].  exp is taken of fp32 values as 2^((l - m) log2e): the
+// is known already) it writes e = exp(l - m) as bf16 to C (ce_store) and the row's sum of e over a quarter of BLOCK_N
+// columns, without the target's, to ce_part[slice][row].  exp is taken of fp32 values as 2^((l - m) log2e): the
 // difference first, which is exact for logits near the reference however large both are.  (One multiply-add less per logit
 // as 2^(l log2e - m log2e), but the rounding of m log2e, common to the row, is 4 % of e at m = 2^20.)  Nothing is rounded to
 // fewer bits before that, and e keeps bf16's relative precision however small it is.  Columns past N and
@@ -2046,7 +2046,7 @@ extern "C" int olb_gemm_bf16(const olb_gemm_desc* d, cudaStream_t stream) {
     if (rc) return rc;
     p.c_tma = 1;
   } else if (epi == OLB_EPI_CE) {
-    if (p.ce_store && d->ldc < (d->N + 63) / 64 * 64) return -18;  // whole chunks of 64 columns are written
+    if (p.ce_store && d->ldc < (d->N + 63) / 64 * 64) return -18;  // whole chunks of 16 or 32 columns are written; rows of 128 bytes
   } else if (!d->accumulate) {
     const uint64_t esz = d->out_fp32 ? 4 : 2;
     uint64_t rows = d->M;

@@ -101,10 +101,10 @@ typedef struct {
   float* tail_part;
   // Cross-entropy product (epilogue == OLB_EPI_CE; DENSE, K-major operands): A = hidden states, B = the head's weight
   // [N, K] with any number of rows N.  Row r has its target in ce_targets[r] (outside [0, N): no target) and a reference
-  // ce_ref[r]; with l the logits, enlarged by ce_grow[r] (> 0) of themselves, C (may be NULL) receives exp(l - ref) as bf16, zeros for rows without a target and up to
-  // the next multiple of 32 columns, and ce_part[i * ce_part_ld + r] (may be NULL) the sum of exp(l - ref) over the i-th
-  // of olb_gemm_ce_slices(M, N) slices of the columns without the target's column.  ce_flags (may be NULL; 1 + ceil(M / 128) ints and ce_max M words, all
-  // zero): a row whose largest logit exceeds its reference by more than 40 has it recorded in ce_max and its block of
+  // ce_ref[r]; with l the logits, enlarged by ce_grow[r] (> 0) of themselves, C (may be NULL; ldc at least N rounded up to 64)
+  // receives exp(l - ref) as bf16, zeros for rows without a target and, up to the next multiple of 16 or 32, for columns past
+  // N, and ce_part[i * ce_part_ld + r] (may be NULL) the sum of exp(l - ref) over the i-th of olb_gemm_ce_slices(M, N) slices
+  // of the columns without the target's column.  ce_flags (may be NULL; 1 + ceil(M / 128) ints and ce_max M words, all zero): a row whose largest logit exceeds its reference by more than 40 has it recorded in ce_max and its block of
   // 128 rows flagged.  ce_repair: the same product for the flagged blocks alone, rows with a recorded maximum against that.
   // With ce_v_total, B holds rows [ce_v0, ce_v0 + N) of a vocabulary of that many and targets count in the whole of it.
   const long long* ce_targets;
@@ -115,9 +115,9 @@ typedef struct {
   long long ce_part_ld;
   int* ce_flags;
   int ce_repair;
-  // OLB_EPI_CE or OLB_EPI_ROWSCALE, C written and not read: start while the launch before this one on the stream is still running, if that allows
-  // it; only the epilogue (row_scale, ce_*, the stores to C) waits for its end.  For a launch whose A and B do not come from
-  // the one before it.  The launch after this one may start early in turn.
+  // OLB_EPI_CE or OLB_EPI_ROWSCALE, C written and not read: start while the launch before this one on the stream is still
+  // running, if that allows it; only the epilogue (row_scale, ce_*, the stores to C) waits for its end.  For a launch whose A
+  // and B do not come from the one before it.  The launch after this one may start early in turn.
   int overlap;
   int wide_tiles;            // DENSE: CTA-pair tiles also for an N below 2048 that is no multiple of 256, where they waste
                              // at most an eighth of it
@@ -244,9 +244,9 @@ int olb_ce_partial_bwd(const void* logits, long long ldl, const long long* label
 
 // ---------------------------------------------------------------- cross entropy from hidden states (linear_ce.cu)
 // The passes around the OLB_EPI_CE product; `rows` is one piece of the batch (see linear_ce.cu for the formulas).
-// ref[r] = x_r . w_t (fp32) for rows with a target t in [0, V), else 0; grow[r]: the product's ce_grow; zeroes ce_max [rows], ce_flags
-// [1 + ceil(rows / 128)] and *ticket.  With count: count[0] = number of all_targets [n_all] in [0, V) (as fp32, rounded
-// above 2^24), count[1] = 1 / that (0 when there are none).  A product launched next with `overlap` starts under this.
+// ref[r] = x_r . w_t (fp32) for rows with a target t in [0, V), else 0; grow[r]: the product's ce_grow; zeroes ce_max
+// [rows], ce_flags [1 + ceil(rows / 128)] and *ticket.  With count: count[0] = number of all_targets [n_all] in [0, V) (as
+// fp32, rounded above 2^24), count[1] = 1 / that (0 when there are none).  A product launched next with `overlap` starts under this.
 int olb_lce_prep(const void* x, long long ldx, const void* w, long long ldw, const long long* targets, int rows, int H,
                  int V, float* ref, float* grow, unsigned* ce_max, int* ce_flags, unsigned* ticket, const long long* all_targets,
                  long long n_all, float* count, cudaStream_t stream);
@@ -254,8 +254,8 @@ int olb_lce_prep(const void* x, long long ldx, const void* w, long long ldw, con
 // sum[r] (of the exponentials without the target's), base[r] (what they are relative to) and inv_z[r] = 1 / (sum and the
 // target's), and with E (the exponentials, row stride lde): the target's entry of E, and
 // factor[r] such that factor[r] * E[r, :] is the row's gradient (times *scale when scale is not NULL); xs (may be NULL):
-// bf16(factor[r] * x[r, :]).  total (may be NULL): sum of loss_all[0, n_all) times *total_scale (NULL: 1), taken by
-// the last block through *ticket.
+// bf16(factor[r] * x[r, :]).  total (may be NULL): sum of loss_all[0, n_all) divided by *total_scale (NULL: 1), taken
+// by the last block through *ticket.
 typedef struct {
   const float* part;
   long long part_ld;

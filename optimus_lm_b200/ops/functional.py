@@ -988,6 +988,12 @@ def linear_cross_entropy(x, weight, targets, reduction="mean", max_workspace=1 <
     (16384 tokens x 2048 against 50304, peak memory above the inputs and time: 2 GiB allowed 1.87 GiB, 7.4 to 7.9 ms; 1 GiB
     1.29 GiB, 7.8 to 8.1; 512 MiB 0.91 GiB, 8.3; 128 MiB 0.57 GiB, 10.7; over the logits 1.79 GiB, 7.5.)
 
+    Precision: logits, their exponentials' sums and the loss are fp32 (tensor-core sums of bf16 products).  The exponentials
+    are rounded to bf16 for the gradient products, the target's entry of each row with its rounding passed on to the rest
+    of the row, and ``x`` times the row's factor once more for the weight's gradient; gradients are summed in fp32 and rounded at
+    the end (``x``'s twice for a batch in pieces, unless the incoming gradient is a power of two).  Their error against
+    64 bits is 0.0017 to 0.0023 of their norm; the rounding at the end alone is 0.0017.
+
     The kernel path takes bf16 CUDA tensors with ``H % 8 == 0``; other inputs take the plain one.  Reference: the
     ``lm_head`` of optimus/models/olmoe/modeling_olmoe.py:502-524 and ``F.cross_entropy`` on its logits."""
     code = _LCE_REDUCTIONS.get(reduction)
