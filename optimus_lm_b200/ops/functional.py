@@ -985,8 +985,9 @@ def linear_cross_entropy(x, weight, targets, reduction="mean", max_workspace=1 <
     the batch in pieces and compute the gradients in the forward, if an fp32 ``[V, H]`` buffer for the weight's gradient fits
     the bound as well (without one: the exponentials of 256 positions); if it does not, and for ``"none"``, the backward
     computes the logits again in pieces of the vocabulary (a third more work, and an fp32 buffer of ``x``'s shape).
-    (16384 tokens x 2048 against 50304, peak memory above the inputs and time: 2 GiB allowed 1.87 GiB, 7.4 to 7.9 ms; 1 GiB
-    1.29 GiB, 7.8 to 8.1; 512 MiB 0.91 GiB, 8.3; 128 MiB 0.57 GiB, 10.7; over the logits 1.79 GiB, 7.5.)
+    (16384 tokens x 2048 against 50304, peak memory above the inputs and time, B200s under their power cap: 2 GiB allowed
+    1.87 GiB, 8.1 to 8.4 ms; 1 GiB 1.29 GiB, 7.7 to 8.4; 512 MiB 0.91 GiB, 8.5; 128 MiB 0.57 GiB, 11.0; over the logits
+    1.79 GiB, 7.8 to 9.5.  ``"none"`` with 2 GiB 7.9 to 8.2 ms, with 1 GiB 1.22 GiB and 10.1 to 10.4.)
 
     Precision: logits, their exponentials' sums and the loss are fp32 (tensor-core sums of bf16 products).  The exponentials
     are rounded to bf16 for the gradient products, the target's entry of each row with its rounding passed on to the rest
