@@ -965,8 +965,10 @@ def linear_cross_entropy_reference(x, weight, targets, reduction="mean"):
     """``cross_entropy(x @ weight.T, targets)`` in fp32 with targets outside ``[0, V)`` ignored."""
     V = weight.shape[0]
     flat = targets.reshape(-1).long()
-    flat = torch.where((flat >= 0) & (flat < V), flat, torch.full_like(flat, -100))
-    logits = F.linear(x.reshape(-1, x.shape[-1]).float(), weight.float())
+    live = (flat >= 0) & (flat < V)
+    flat = torch.where(live, flat, torch.full_like(flat, -100))
+    rows = torch.where(live[:, None], x.reshape(-1, x.shape[-1]).float(), 0.0)   # what an ignored row holds reaches no gradient
+    logits = F.linear(rows, weight.float())
     loss = F.cross_entropy(logits, flat, ignore_index=-100, reduction=reduction)
     return loss.view(targets.shape) if reduction == "none" else loss
 

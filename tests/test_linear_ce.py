@@ -61,3 +61,18 @@ def test_shifted_form_takes_integer_labels(bad):
     with pytest.raises(ValueError, match="integers"):
         OF.shifted_linear_cross_entropy(x.view(4, 6, 16), w, torch.ones(4, 6).to(bad))
     assert torch.isfinite(OF.shifted_linear_cross_entropy(x.view(4, 6, 16), w, torch.ones(4, 6, dtype=torch.int32)))
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_ignored_rows_may_hold_anything(reduction, bad):
+    x, w, t = problem()
+    clean = x.detach().clone().requires_grad_()
+    with torch.no_grad():
+        x[3], x[5, 2], x[6] = bad, bad, -bad
+        clean[3], clean[5], clean[6] = 0.0, 0.0, 0.0
+    got, want = OF.linear_cross_entropy(x, w, t, reduction), OF.linear_cross_entropy(clean, w, t, reduction)
+    assert torch.equal(got, want)
+    v = torch.ones_like(got)
+    for a, b in zip(torch.autograd.grad(got, (x, w), v), torch.autograd.grad(want, (clean, w), v)):
+        assert torch.equal(a, b)
