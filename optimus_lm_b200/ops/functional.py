@@ -1163,6 +1163,7 @@ def sum_of_squares(t: torch.Tensor, scale: float = 1.0, out: Optional[torch.Tens
 
 
 def _grad_norm_reference(grads, norm_type):
+    grads = [g.detach().abs() if g.is_complex() else g for g in grads]
     if norm_type == math.inf:
         return torch.stack([g.detach().abs().max().float() for g in grads]).max()
     return torch.stack([g.detach().double().square().sum() for g in grads]).sum().sqrt().float()
@@ -1241,9 +1242,11 @@ def clip_grad_norm_(grads, max_norm: float, norm_type: float = 2.0) -> torch.Ten
             return norm
     with torch.no_grad():
         norm = grad_norm(grads, norm_type)
+        if not all(g.is_floating_point() or g.is_complex() for g in grads):
+            raise TypeError("gradients to be scaled must be floating-point or complex tensors")
         copies = {i: grads[i].clone() for i in _check_scalable(grads)}
         factor = torch.clamp(max_norm / (norm + 1e-6), max=1.0)
         for i, g in enumerate(grads):
             old = copies.get(i, g)
-            g.copy_(old.float() * factor if g.dtype != torch.float64 else old * factor)
+            g.copy_(old * factor if g.is_complex() or g.dtype == torch.float64 else old.float() * factor)
     return norm

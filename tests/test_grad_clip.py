@@ -75,3 +75,20 @@ def test_shared_memory_is_refused_when_scaled(dtype):
     v = torch.full((10,), 2.0, dtype=dtype)
     norm = OF.clip_grad_norm_([v, v[::3]], 1.0)
     assert torch.allclose(v.float(), torch.full((10,), 2 / (norm.item() + 1e-6)), rtol=2.0 ** -10)
+
+
+@pytest.mark.parametrize("norm_type", [2.0, math.inf])
+def test_complex_and_integer_types(norm_type):
+    g = torch.Generator().manual_seed(2)
+    grads = [torch.complex(torch.randn(7, generator=g), torch.randn(7, generator=g)), torch.randn(5, generator=g)]
+    before = [x.clone() for x in grads]
+    want = torch.linalg.vector_norm(torch.cat([x.abs().double() for x in grads]), norm_type)
+    assert OF.grad_norm(grads, norm_type).item() == pytest.approx(want.item(), rel=1e-6)
+    OF.clip_grad_norm_(grads, 0.5, norm_type)
+    for a, b in zip(grads, before):
+        assert torch.allclose(a, b * (0.5 / (want.item() + 1e-6)), rtol=1e-6)
+    whole = [torch.tensor([3, 4]), torch.zeros(2)]
+    assert OF.grad_norm(whole, norm_type).item() == (5 if norm_type == 2 else 4)
+    with pytest.raises(TypeError, match="floating"):   # whole numbers cannot be scaled
+        OF.clip_grad_norm_(whole, 0.5, norm_type)
+    assert whole[0].tolist() == [3, 4]
