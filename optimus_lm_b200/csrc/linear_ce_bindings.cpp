@@ -90,8 +90,8 @@ void rowscale_product(const Problem& p, olb_gemm_desc& d, const char* what) {
 
 // e = exp(l - ref) of some rows and columns [v0, v0 + cols) of the vocabulary (and the sums of their tiles), then of the
 // row blocks that need another reference.
-void product(const Problem& p, int64_t r0, int64_t rows, int64_t v0, int64_t cols, const float* ref, const float* grow, unsigned* top, int* flags,
-             float* part, int64_t part_ld, void* E, int64_t lde, bool behind_prep) {
+void product(const Problem& p, int64_t r0, int64_t rows, int64_t v0, int64_t cols, const float* ref, const float* grow,
+             unsigned* top, int* flags, float* part, int64_t part_ld, void* E, int64_t lde, bool behind_prep) {
   olb_gemm_desc d{};
   d.A = row_ptr(p.x, r0);
   d.B = row_ptr(p.w, v0);

@@ -104,8 +104,9 @@ typedef struct {
   // ce_ref[r]; with l the logits, enlarged by ce_grow[r] (> 0) of themselves, C (may be NULL; ldc at least N rounded up to 64)
   // receives exp(l - ref) as bf16, zeros for rows without a target and, up to the next multiple of 16 or 32, for columns past
   // N, and ce_part[i * ce_part_ld + r] (may be NULL) the sum of exp(l - ref) over the i-th of olb_gemm_ce_slices(M, N) slices
-  // of the columns without the target's column.  ce_flags (may be NULL; 1 + ceil(M / 128) ints and ce_max M words, all zero): a row whose largest logit exceeds its reference by more than 40 has it recorded in ce_max and its block of
-  // 128 rows flagged.  ce_repair: the same product for the flagged blocks alone, rows with a recorded maximum against that.
+  // of the columns without the target's column.  ce_flags (may be NULL; 1 + ceil(M / 128) ints and ce_max M words, all zero):
+  // a row whose largest logit exceeds its reference by more than 40 has it recorded in ce_max and its block of 128 rows
+  // flagged.  ce_repair: the same product for the flagged blocks alone, rows with a recorded maximum against that.
   // With ce_v_total, B holds rows [ce_v0, ce_v0 + N) of a vocabulary of that many and targets count in the whole of it.
   const long long* ce_targets;
   int ce_v0, ce_v_total;
